@@ -69,12 +69,13 @@ def _run(cmd):
 
 
 def build_lib() -> Path:
-    """The device code is seven translation units (the decode kernels once per element type and
-    transform switch, the rest), compiled side by side into objects under build/, then linked
-    with the host sources."""
+    """The device code is eleven translation units (the decode kernels once per element type and
+    transform switch, the tree kernels once per element type, the moves of cache slots, the rest),
+    compiled side by side into objects under build/, then linked with the host sources."""
     hipcc = ROCM / "bin" / "hipcc"
     units = ["ffa_decode_f16.hip", "ffa_decode_bf16.hip", "ffa_decode_f32.hip", "ffa_decode_f16_xform.hip",
-             "ffa_decode_bf16_xform.hip", "ffa_decode_f32_xform.hip", "ffa_kernels.hip"]
+             "ffa_decode_bf16_xform.hip", "ffa_decode_f32_xform.hip", "ffa_tree_f16.hip", "ffa_tree_bf16.hip",
+             "ffa_tree_f32.hip", "ffa_slots.hip", "ffa_kernels.hip"]
     obj_dir = PKG_DIR / "build"
     obj_dir.mkdir(exist_ok=True)
     flags = [f for f in HIPCC_FLAGS if f != "-shared"]
@@ -87,8 +88,8 @@ def build_lib() -> Path:
     if failed:
         raise RuntimeError(f"hipcc failed on {failed}")
     objs = [obj_dir / (u + ".o") for u in units]
-    _run([hipcc, *HIPCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", *objs, CSRC / "ffa_api.cpp", CSRC / "ffa_plan.cpp",
-          "-o", LIB_PATH])
+    _run([hipcc, *HIPCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", *objs, CSRC / "ffa_api.cpp", CSRC / "ffa_cache_ops.cpp",
+          CSRC / "ffa_plan.cpp", "-o", LIB_PATH])
     LIB_HASH.write_text(lib_source_hash())
     return LIB_PATH
 

@@ -26,6 +26,7 @@ STATUS_NAMES = {
     4: "FFA_ERR_SHAPE", 5: "FFA_ERR_TIMESTEP", 6: "FFA_ERR_ALIGNMENT", 7: "FFA_ERR_WORKSPACE",
     8: "FFA_ERR_PLAN", 9: "FFA_ERR_TOO_LONG", 10: "FFA_ERR_PROB_THRESH", 11: "FFA_ERR_LAUNCH",
     12: "FFA_ERR_NO_DEVICE", 13: "FFA_ERR_SCRATCH_LIMIT", 14: "FFA_ERR_TRANSFORM", 15: "FFA_ERR_BEAM",
+    16: "FFA_ERR_TREE", 17: "FFA_ERR_EVICT", 18: "FFA_ERR_OVERLAP",
 }
 globals().update({name: code for code, name in STATUS_NAMES.items()})   # FFA_OK, FFA_ERR_* as ints
 
@@ -59,10 +60,19 @@ class BeamIndirection(C.Structure):
     _fields_ = [("cache_indir", C.c_void_p), ("beam_width", C.c_int32)]
 
 
+class TreeTokens(C.Structure):
+    """struct ffa_tree_tokens."""
+    _fields_ = [("tokens", C.c_int32), ("q_head_num", C.c_int32), ("parents", C.c_void_p), ("first_keys", C.c_void_p),
+                ("lengths", C.c_void_p), ("counts", C.c_void_p), ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3),
+                ("v_stride", C.c_int64 * 3), ("out_stride", C.c_int64 * 3)]
+
+
 _vp, _i, _f, _sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
 _PLAN_P = C.POINTER(LaunchPlan)
 _TT_P = C.POINTER(TokenTransform)
 _BI_P = C.POINTER(BeamIndirection)
+_TR_P = C.POINTER(TreeTokens)
+_VPP = C.POINTER(C.c_void_p)       # host arrays of device pointers
 
 # name -> (restype, argtypes); one entry per declaration in include/ffa_c_api.h
 SIGNATURES = {
@@ -86,6 +96,13 @@ SIGNATURES = {
                               _BI_P, _vp, _sz, _vp]),
     "ffa_attention_static_scratch": (_i, [_i, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f,
                                           _PLAN_P, _i, _TT_P, _BI_P, _vp]),
+    "ffa_tree_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
+    "ffa_attention_tree": (_i, [_i, _i, _i, _i, _i, _f, _i, _TR_P, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ffa_commit_tree": (_i, [_i, _i, _VPP, _VPP, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp]),
+    "ffa_weights_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "ffa_attention_weights": (_i, [_i, _i, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                   _sz, _vp]),
+    "ffa_evict": (_i, [_i, _i, _VPP, _VPP, _VPP, _VPP, _VPP, _VPP, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "ffa_load_floor": (_i, [_i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _PLAN_P, _vp, _vp]),
 }
 

@@ -1,0 +1,277 @@
+// C ABI of the operators next to the decode step (attention of a group of tokens, the
+// weight-summing step, path commit, eviction): argument validation, planning, workspace carving.
+// Pure host C++; the kernels live in ffa_tree_kernels.h and ffa_slots.hip.
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "ffa_c_api.h"
+#include "ffa_cache_ops.h"
+
+using namespace ffa;
+
+namespace {
+
+bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+int compute_units() {
+    const int cus = query_compute_units();
+    return cus > 0 ? cus : 256;
+}
+
+int check_cache_shape(int precision, int B, int H, int Dh, int Lmax) {
+    if (elem_bytes(precision) == 0) return FFA_ERR_DTYPE;
+    if (Dh != 64 && Dh != 80 && Dh != 128 && Dh != 256) return FFA_ERR_HEAD_DIM;
+    if (B <= 0 || H <= 0 || Lmax <= 0) return FFA_ERR_SHAPE;
+    // Four chunk rows of a K cache are addressed with 32 bits from their first byte.
+    if ((long long)B * H > (1ll << 20) || Lmax > (1 << 25)) return FFA_ERR_SHAPE;
+    return FFA_OK;
+}
+
+// Weight-summing step: scores of the cached keys in whole wave tiles, the new token's behind them.
+int score_stride_of(int t) { return (int)align_up((size_t)t, 32) + 32; }
+
+struct TreeSizes {
+    size_t acc = 0, ml = 0, scores = 0;
+    size_t total() const { return acc + ml + scores; }
+};
+
+// With n_splits the most pieces the plan takes up to this t, which grows with t.
+TreeSizes tree_sizes(int pairs, int rows, int head_dim, int n_splits, bool scores, int t) {
+    TreeSizes s;
+    if (n_splits > 1) s.acc = align_up((size_t)pairs * n_splits * rows * head_dim * sizeof(float), 256);
+    if (n_splits > 1 || scores) s.ml = align_up((size_t)pairs * n_splits * rows * 2 * sizeof(float), 256);
+    if (scores) s.scores = align_up((size_t)pairs * rows * score_stride_of(t) * sizeof(float), 256);
+    return s;
+}
+
+int most_splits(int precision, int pairs, int row_blocks, int t, int cus) {
+    const int tiles = ceil_div(t, tree_tile_keys(precision));
+    // About four workgroups a CU hide the memory's latency; a piece has two tiles a wave at least,
+    // or its prologue and the merge cost more than the tiles.
+    const int want = ceil_div(4 * cus, pairs * row_blocks);
+    return std::max(1, std::min({want, tiles / (2 * kTreeWaves), 128}));
+}
+
+int row_blocks_of(int rows, int head_dim) {
+    // Row tiles a wave can hold: Dh = 256 fills the registers with two.
+    return ceil_div(ceil_div(rows, 16), head_dim == 256 ? 2 : 4);
+}
+
+int run_tree(int precision, int head_dim, TreeParams& P, void* workspace, size_t workspace_bytes, void* stream) {
+    const int pairs = P.B * P.H;
+    const TreePlan plan = plan_tree(precision, pairs, P.rows, head_dim, P.t, compute_units());
+    const bool scores = P.key_weights != nullptr;
+    const int most = most_splits(precision, pairs, plan.row_blocks, P.t, compute_units());
+    const TreeSizes s = tree_sizes(pairs, P.rows, head_dim, most, scores, P.t);
+    if (s.total() > 0) {
+        if (workspace == nullptr || workspace_bytes < s.total()) return FFA_ERR_WORKSPACE;
+        if (!aligned(workspace, 16)) return FFA_ERR_ALIGNMENT;
+    }
+    char* base = static_cast<char*>(workspace);
+    P.ws_acc = reinterpret_cast<float*>(base);
+    P.ws_ml = reinterpret_cast<float*>(base + s.acc);
+    P.ws_scores = scores ? reinterpret_cast<float*>(base + s.acc + s.ml) : nullptr;
+    P.score_stride = score_stride_of(P.t);
+    P.n_splits = plan.n_splits;
+    P.tiles_per_split = plan.tiles_per_split;
+    P.row_blocks = plan.row_blocks;
+    return launch_tree(precision, head_dim, P, plan, stream);
+}
+
+size_t tree_workspace(int precision, int B, int H, int Hq, int Dh, int tokens, int t, bool scores) {
+    if (check_cache_shape(precision, B, H, Dh, 1) != FFA_OK || Hq <= 0 || Hq % H != 0 || tokens < 1 ||
+        tokens > FFA_MAX_TREE_TOKENS || t < 0)
+        return 0;
+    const long long rows = (long long)(Hq / H) * tokens;
+    if (rows > (1 << 20)) return 0;
+    const int n = most_splits(precision, B * H, row_blocks_of((int)rows, Dh), t, compute_units());
+    return tree_sizes(B * H, (int)rows, Dh, n, scores, t).total();
+}
+
+bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + nb && y < x + na;
+}
+
+}  // namespace
+
+namespace ffa {
+
+TreePlan plan_tree(int precision, int pairs, int rows, int head_dim, int t, int cus) {
+    TreePlan p;
+    p.row_blocks = row_blocks_of(rows, head_dim);
+    p.row_tiles = ceil_div(ceil_div(rows, 16), p.row_blocks);
+    const int tiles = ceil_div(t, tree_tile_keys(precision));
+    const int n = most_splits(precision, pairs, p.row_blocks, t, cus);
+    p.tiles_per_split = std::max(1, ceil_div(tiles, n));
+    p.n_splits = std::max(1, ceil_div(tiles, p.tiles_per_split));
+    return p;
+}
+
+}  // namespace ffa
+
+extern "C" {
+
+size_t ffa_tree_workspace_bytes(int precision, int batch_size, int head_num, int q_head_num, int head_dim, int tokens,
+                                int t) {
+    return tree_workspace(precision, batch_size, head_num, q_head_num, head_dim, tokens, t, false);
+}
+
+size_t ffa_weights_workspace_bytes(int precision, int batch_size, int head_num, int q_head_num, int head_dim, int t) {
+    return tree_workspace(precision, batch_size, head_num, q_head_num, head_dim, 1, t, true);
+}
+
+int ffa_attention_tree(int precision, int batch_size, int head_num, int head_dim, int max_seq_len, float softmax_scale,
+                       int t, const ffa_tree_tokens* tokens, const void* q, const void* k, const void* v, void* k_cache,
+                       void* v_cache, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+    const int st = check_cache_shape(precision, batch_size, head_num, head_dim, max_seq_len);
+    if (st != FFA_OK) return st;
+    if (t < 0 || t >= max_seq_len) return FFA_ERR_TIMESTEP;
+    if (!tokens || !q || !k || !v || !k_cache || !v_cache || !out) return FFA_ERR_NULL_POINTER;
+    const int n = tokens->tokens, Hq = tokens->q_head_num;
+    if (n < 1 || n > FFA_MAX_TREE_TOKENS || n > max_seq_len - t || Hq <= 0 || Hq % head_num != 0) return FFA_ERR_TREE;
+    if ((long long)batch_size * Hq * n > (1ll << 24)) return FFA_ERR_SHAPE;
+    const int unit = 16 / elem_bytes(precision);
+    for (int i = 0; i < 3; ++i)
+        if (tokens->q_stride[i] % unit || tokens->k_stride[i] % unit || tokens->v_stride[i] % unit ||
+            tokens->out_stride[i] % unit)
+            return FFA_ERR_TREE;
+    for (const void* p : {q, k, v, (const void*)k_cache, (const void*)v_cache, (const void*)out})
+        if (!aligned(p, 16)) return FFA_ERR_ALIGNMENT;
+    for (const int32_t* p : {tokens->parents, tokens->first_keys, tokens->lengths, tokens->counts})
+        if (!aligned(p, 4)) return FFA_ERR_ALIGNMENT;
+    TreeParams P = {};
+    P.q = q; P.k = k; P.v = v;
+    P.k_cache = k_cache; P.v_cache = v_cache; P.out = out;
+    P.parents = tokens->parents; P.first_keys = tokens->first_keys;
+    P.lengths = tokens->lengths; P.counts = tokens->counts;
+    for (int i = 0; i < 3; ++i) {
+        P.q_stride[i] = tokens->q_stride[i]; P.k_stride[i] = tokens->k_stride[i];
+        P.v_stride[i] = tokens->v_stride[i]; P.out_stride[i] = tokens->out_stride[i];
+    }
+    P.B = batch_size; P.H = head_num; P.G = Hq / head_num; P.tokens = n; P.rows = P.G * n;
+    P.Lmax = max_seq_len; P.t = t;
+    P.scale_log2e = softmax_scale * 1.4426950408889634f;
+    return run_tree(precision, head_dim, P, workspace, workspace_bytes, stream);
+}
+
+int ffa_attention_weights(int precision, int batch_size, int head_num, int q_head_num, int head_dim, int max_seq_len,
+                          float softmax_scale, int t, const void* q, const void* k, const void* v, void* k_cache,
+                          void* v_cache, void* out, float* key_weights, const int32_t* first_keys,
+                          const int32_t* lengths, void* workspace, size_t workspace_bytes, void* stream) {
+    const int st = check_cache_shape(precision, batch_size, head_num, head_dim, max_seq_len);
+    if (st != FFA_OK) return st;
+    if (t < 0 || t >= max_seq_len) return FFA_ERR_TIMESTEP;
+    if (!q || !k || !v || !k_cache || !v_cache || !out || !key_weights) return FFA_ERR_NULL_POINTER;
+    if (q_head_num <= 0 || q_head_num % head_num != 0) return FFA_ERR_TREE;
+    if ((long long)batch_size * q_head_num > (1ll << 24)) return FFA_ERR_SHAPE;
+    for (const void* p : {q, k, v, (const void*)k_cache, (const void*)v_cache, (const void*)out})
+        if (!aligned(p, 16)) return FFA_ERR_ALIGNMENT;
+    if (!aligned(key_weights, 4) || !aligned(first_keys, 4) || !aligned(lengths, 4)) return FFA_ERR_ALIGNMENT;
+    TreeParams P = {};
+    P.q = q; P.k = k; P.v = v;
+    P.k_cache = k_cache; P.v_cache = v_cache; P.out = out;
+    P.first_keys = first_keys; P.lengths = lengths;
+    P.key_weights = key_weights;
+    const long long qs[3] = {(long long)q_head_num * head_dim, head_dim, 0};
+    const long long ks[3] = {(long long)head_num * head_dim, head_dim, 0};
+    for (int i = 0; i < 3; ++i) {
+        P.q_stride[i] = P.out_stride[i] = qs[i];
+        P.k_stride[i] = P.v_stride[i] = ks[i];
+    }
+    P.B = batch_size; P.H = head_num; P.G = q_head_num / head_num; P.tokens = 1; P.rows = P.G;
+    P.Lmax = max_seq_len; P.t = t;
+    P.scale_log2e = softmax_scale * 1.4426950408889634f;
+    return run_tree(precision, head_dim, P, workspace, workspace_bytes, stream);
+}
+
+int ffa_commit_tree(int precision, int n_caches, void* const* k_caches, void* const* v_caches, int batch_size,
+                    int head_num, int head_dim, int max_seq_len, int t, const int32_t* path, int path_len,
+                    const int32_t* accepted, const int32_t* lengths, void* stream) {
+    const int st = check_cache_shape(precision, batch_size, head_num, head_dim, max_seq_len);
+    if (st != FFA_OK) return st;
+    if (n_caches < 0) return FFA_ERR_SHAPE;
+    if (t < 0 || t >= max_seq_len) return FFA_ERR_TIMESTEP;
+    if (path_len < 1 || path_len > FFA_MAX_TREE_TOKENS || path_len > max_seq_len - t) return FFA_ERR_TREE;
+    if (!path || !accepted || (n_caches > 0 && (!k_caches || !v_caches))) return FFA_ERR_NULL_POINTER;
+    if (!aligned(path, 4) || !aligned(accepted, 4) || !aligned(lengths, 4)) return FFA_ERR_ALIGNMENT;
+    for (int i = 0; i < n_caches; ++i) {
+        if (!k_caches[i] || !v_caches[i]) return FFA_ERR_NULL_POINTER;
+        if (!aligned(k_caches[i], 16) || !aligned(v_caches[i], 16)) return FFA_ERR_ALIGNMENT;
+    }
+    for (int i0 = 0; i0 < n_caches; i0 += kSlotCaches) {
+        CommitParams P = {};
+        P.n_caches = std::min(kSlotCaches, n_caches - i0);
+        for (int i = 0; i < P.n_caches; ++i) {
+            P.k[i] = k_caches[i0 + i];
+            P.v[i] = v_caches[i0 + i];
+        }
+        P.path = path; P.accepted = accepted; P.lengths = lengths;
+        P.path_len = path_len; P.B = batch_size; P.H = head_num; P.Lmax = max_seq_len; P.t = t;
+        const int rc = launch_commit(P, head_dim, elem_bytes(precision), stream);
+        if (rc != FFA_OK) return rc;
+    }
+    return FFA_OK;
+}
+
+int ffa_evict(int precision, int n_caches, const void* const* k_src, const void* const* v_src,
+              const float* const* w_src, void* const* k_dst, void* const* v_dst, float* const* w_dst, int batch_size,
+              int head_num, int head_dim, int src_max_seq_len, int dst_max_seq_len, int t, int keep, int recent,
+              const int32_t* first_keys, const int32_t* lengths, int32_t* kept, void* stream) {
+    int st = check_cache_shape(precision, batch_size, head_num, head_dim, src_max_seq_len);
+    if (st == FFA_OK) st = check_cache_shape(precision, batch_size, head_num, head_dim, dst_max_seq_len);
+    if (st != FFA_OK) return st;
+    if (n_caches < 0) return FFA_ERR_SHAPE;
+    if (t < 0 || t > src_max_seq_len) return FFA_ERR_TIMESTEP;
+    if (keep < 1 || keep > dst_max_seq_len || recent < 0 || recent > keep) return FFA_ERR_EVICT;
+    if (n_caches == 0) return FFA_OK;
+    if (!k_src || !v_src || !w_src || !k_dst || !v_dst || !w_dst || !kept) return FFA_ERR_NULL_POINTER;
+    if (!aligned(first_keys, 4) || !aligned(lengths, 4) || !aligned(kept, 4)) return FFA_ERR_ALIGNMENT;
+    const size_t pairs = (size_t)batch_size * head_num;
+    const size_t src_kv = pairs * src_max_seq_len * head_dim * elem_bytes(precision), src_w = pairs * src_max_seq_len * 4;
+    const size_t dst_kv = pairs * dst_max_seq_len * head_dim * elem_bytes(precision), dst_w = pairs * dst_max_seq_len * 4;
+    for (int i = 0; i < n_caches; ++i) {
+        if (!k_src[i] || !v_src[i] || !w_src[i] || !k_dst[i] || !v_dst[i] || !w_dst[i]) return FFA_ERR_NULL_POINTER;
+        for (const void* p : {k_src[i], v_src[i], (const void*)k_dst[i], (const void*)v_dst[i]})
+            if (!aligned(p, 16)) return FFA_ERR_ALIGNMENT;
+        if (!aligned(w_src[i], 4) || !aligned(w_dst[i], 4)) return FFA_ERR_ALIGNMENT;
+    }
+    // Every target against every other buffer of the call: its own source may be the same buffer of the same shape.
+    const bool same_shape = src_max_seq_len == dst_max_seq_len;
+    for (int i = 0; i < n_caches; ++i) {
+        const void* dst[3] = {k_dst[i], v_dst[i], w_dst[i]};
+        for (int a = 0; a < 3; ++a) {
+            const size_t na = a == 2 ? dst_w : dst_kv;
+            for (int j = 0; j < n_caches; ++j) {
+                const void* src2[3] = {k_src[j], v_src[j], w_src[j]};
+                const void* dst2[3] = {k_dst[j], v_dst[j], w_dst[j]};
+                for (int b = 0; b < 3; ++b) {
+                    const bool own = i == j && a == b;
+                    if (!(own && same_shape && src2[b] == dst[a]) && overlap(dst[a], na, src2[b], b == 2 ? src_w : src_kv))
+                        return FFA_ERR_OVERLAP;
+                    if (!own && overlap(dst[a], na, dst2[b], b == 2 ? dst_w : dst_kv)) return FFA_ERR_OVERLAP;
+                }
+            }
+            if (overlap(dst[a], na, kept, (size_t)n_caches * pairs * keep * 4)) return FFA_ERR_OVERLAP;
+        }
+    }
+    for (int i0 = 0; i0 < n_caches; i0 += kSlotCaches) {
+        EvictParams P = {};
+        P.n_caches = std::min(kSlotCaches, n_caches - i0);
+        for (int i = 0; i < P.n_caches; ++i) {
+            P.k_src[i] = k_src[i0 + i]; P.v_src[i] = v_src[i0 + i]; P.w_src[i] = w_src[i0 + i];
+            P.k_dst[i] = k_dst[i0 + i]; P.v_dst[i] = v_dst[i0 + i]; P.w_dst[i] = w_dst[i0 + i];
+        }
+        P.first_keys = first_keys; P.lengths = lengths;
+        P.kept = kept + (size_t)i0 * pairs * keep;
+        P.B = batch_size; P.H = head_num; P.src_len = src_max_seq_len; P.dst_len = dst_max_seq_len;
+        P.t = t; P.keep = keep; P.recent = recent;
+        const int rc = launch_evict(P, head_dim, elem_bytes(precision), stream);
+        if (rc != FFA_OK) return rc;
+    }
+    return FFA_OK;
+}
+
+}  // extern "C"

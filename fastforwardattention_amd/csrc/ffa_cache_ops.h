@@ -1,0 +1,72 @@
+// Host-side declarations of the operators next to the decode step: attention of a group of new
+// tokens, the weight-summing decode step, and the moves of cache slots (path commit, eviction).
+#pragma once
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include "ffa_host.h"
+
+namespace ffa {
+
+// ---------------------------------------------------------------------------------------
+// Attention of a group of tokens.  The rows of a (sample, cache head) pair -- its tokens times
+// its G query heads, row = token * G + head -- are cut into blocks of row_tiles * 16; a
+// workgroup of kTreeWaves waves takes one row block over one piece of the keys.
+constexpr int kTreeWaves = 4;
+
+// Keys of one wave tile: two (16-bit) or one (fp32) matrix tiles of 16 keys.
+inline int tree_tile_keys(int precision) { return precision == FFA_PRECISION_F32 ? 16 : 32; }
+
+struct TreePlan {
+    int row_tiles;        // 16-row matrix tiles a wave holds: 1 .. 4
+    int row_blocks;       // workgroups a piece of keys is read by
+    int n_splits;         // pieces of the cached keys
+    int tiles_per_split;  // wave tiles a piece holds
+};
+
+struct TreeParams {
+    const void *q, *k, *v;
+    void *k_cache, *v_cache, *out;
+    const int *parents, *first_keys, *lengths, *counts;
+    long long q_stride[3], k_stride[3], v_stride[3], out_stride[3];  // (sample, head, token), elements
+    float* ws_acc;       // [pairs, n_splits, rows, Dh], or unused with one piece
+    float* ws_ml;        // [pairs, n_splits, rows, 2]: reference exponent and sum
+    float* ws_scores;    // weight-summing step: [pairs, rows, score_stride], else nullptr
+    float* key_weights;  // weight-summing step: [pairs, Lmax], else nullptr
+    int score_stride;
+    int B, H, G, tokens, rows, Lmax, t;
+    float scale_log2e;
+    int n_splits, tiles_per_split, row_blocks;
+};
+
+TreePlan plan_tree(int precision, int pairs, int rows, int head_dim, int t, int cus);
+int launch_tree(int precision, int head_dim, const TreeParams& P, const TreePlan& plan, void* stream);
+int launch_tree_f16(const TreeParams& P, int head_dim, int row_tiles, void* stream);
+int launch_tree_bf16(const TreeParams& P, int head_dim, int row_tiles, void* stream);
+int launch_tree_f32(const TreeParams& P, int head_dim, int row_tiles, void* stream);
+
+// ---------------------------------------------------------------------------------------
+// Moves of cache slots.  Pointers of up to kSlotCaches caches travel in the kernel arguments.
+constexpr int kSlotCaches = 32;
+
+struct CommitParams {
+    void* k[kSlotCaches];
+    void* v[kSlotCaches];
+    const int *path, *accepted, *lengths;
+    int path_len, n_caches, B, H, Lmax, t;
+};
+int launch_commit(const CommitParams& P, int head_dim, int elem_bytes, void* stream);
+
+struct EvictParams {
+    const void *k_src[kSlotCaches], *v_src[kSlotCaches];
+    const float* w_src[kSlotCaches];
+    void *k_dst[kSlotCaches], *v_dst[kSlotCaches];
+    float* w_dst[kSlotCaches];
+    const int *first_keys, *lengths;
+    int* kept;  // [n_caches, B, H, keep]
+    int n_caches, B, H, src_len, dst_len, t, keep, recent;
+};
+int launch_evict(const EvictParams& P, int head_dim, int elem_bytes, void* stream);
+
+}  // namespace ffa

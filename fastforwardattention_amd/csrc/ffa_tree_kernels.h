@@ -1,0 +1,621 @@
+// Attention of a group of new tokens over the decode caches (gfx950, MFMA): drafted trees, chains,
+// and the one-token step that sums attention weights.  Included by one translation unit per
+// element type (ffa_tree_{f16,bf16,f32}.hip).
+//
+// Mathematics.  The rows of a (sample, cache head) pair are its tokens times its G query heads.
+// For a tile of keys:  S^T = K Q^T (keys x rows),  P = 2^(S c - m),  O^T += V^T P^T (dims x rows),
+// l += sum P, with c = softmax_scale * log2(e) and m one reference exponent a row.  Any m cancels
+// in O / l, so m is only moved when a score exceeds it by kSlack: then rows are rescaled so that
+// their largest P is 2^kLift.  Pieces (waves, workgroups) are joined by their (m, l, O).
+//
+// Layout.  No operand passes through LDS.  A 16-byte chunk of a K cache row holds 8 (4) dims of
+// one key, which is what one lane of a 16x16x32 (four 16x16x4) matrix product wants of its left
+// operand.  The product's result has one row of Q a lane (lane % 16) and four keys in its
+// registers, and the second product takes P in that order if V is read in it too: contraction
+// slot (lane group g, j) is key 16 (j / 4) + 4 g + j % 4 of the tile.  V arrives in 16-byte (8-byte
+// for Dh = 64) pieces of a key's row and is turned in registers, two 16-bit halves a v_perm.
+//
+// What bounds it: up to about 200 rows a pair in 16 bits the bytes of the caches (each read once a
+// row block), above that the matrix units.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "ffa_cache_ops.h"
+#include "ffa_device.h"
+
+namespace ffa {
+
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+// Scores may exceed a row's reference exponent by kSlack; a rescaled row starts at 2^kLift.  In
+// fp16 the range of P is what these two set: below 65504 at the top, and a weight of 2^-30 of the
+// row's largest is still above half the smallest number.
+constexpr float kSlack = 15.f, kLift = 6.f;
+
+// Geometry of one element type and head dimension.
+template <typename T, int DH> struct TreeGeo {
+    static constexpr int X = Elem<T>::X;                 // elements of a 16-byte chunk
+    static constexpr int NCH = DH / X;                   // chunks of a row
+    static constexpr int KK = (NCH + 3) / 4;             // chunk groups of a K row, one chunk a lane group
+    static constexpr int NU = X == 8 ? 2 : 1;            // 16-key matrix tiles of a wave tile
+    static constexpr int TK = 16 * NU;                   // keys of a wave tile
+    // A V row is cut into blocks of 16 * E dims, E of them a lane: E = 8 or 4 (16 or 8 bytes), the
+    // last 16 dims of Dh = 80 one by one.
+    static constexpr int E = X == 8 ? (DH >= 128 ? 8 : 4) : 4;
+    static constexpr int NBLK = DH / (16 * E);           // whole blocks
+    static constexpr int TAIL = DH - NBLK * 16 * E;      // 0, or 16
+    static constexpr int DB = DH / 16;                   // 16-dim result tiles
+};
+
+// One chunk of K against one of Q for 16 keys x 16 rows.
+__device__ __forceinline__ f32x4_t mma_qk(const uint4& k, const uint4& q, f32x4_t acc, uint16_t) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, k), __builtin_bit_cast(f16x8_t, q), acc, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_t mma_qk(const uint4& k, const uint4& q, f32x4_t acc, bf16_t) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k), __builtin_bit_cast(bf16x8_t, q), acc, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_t mma_qk(const uint4& k, const uint4& q, f32x4_t acc, float) {
+    const f32x4_t a = __builtin_bit_cast(f32x4_t, k), b = __builtin_bit_cast(f32x4_t, q);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], acc, 0, 0, 0);
+    return acc;
+}
+
+// The weights of one row tile as right operands.  16-bit types: P = hi + lo, hi rounded towards
+// zero, so that the weights are off by 2^-20 (fp16) or 2^-14 (bf16) at most and the result is as
+// good as with fp32 weights after its own rounding to 11 or 8 bits.  lo is kept above zero: 0 * V would turn an infinite
+// V into NaN.  (A NaN weight is NaN in hi; fmaxf makes it tiny in lo.)
+struct PFrag16 { uint4 hi, lo; };
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint32_t* lo, uint16_t) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    *hi = __builtin_bit_cast(uint32_t, h);
+    constexpr float tiny = 5.9604644775390625e-8f;  // 2^-24, the smallest fp16
+    *lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaxf(a - (float)h[0], tiny), fmaxf(b - (float)h[1], tiny)));
+}
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint32_t* lo, bf16_t) {
+    const uint32_t ua = __builtin_bit_cast(uint32_t, a), ub = __builtin_bit_cast(uint32_t, b);
+    *hi = __builtin_amdgcn_perm(ub, ua, 0x07060302);
+    constexpr float tiny = 5.9604644775390625e-8f;
+    const float la = fmaxf(a - __builtin_bit_cast(float, ua & 0xffff0000u), tiny);
+    const float lb = fmaxf(b - __builtin_bit_cast(float, ub & 0xffff0000u), tiny);
+    *lo = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, lb), __builtin_bit_cast(uint32_t, la), 0x07060302);
+}
+
+template <typename T> __device__ __forceinline__ PFrag16 split_weights(const float (&p)[8], T tag) {
+    PFrag16 f;
+    split_pair(p[0], p[1], &f.hi.x, &f.lo.x, tag);
+    split_pair(p[2], p[3], &f.hi.y, &f.lo.y, tag);
+    split_pair(p[4], p[5], &f.hi.z, &f.lo.z, tag);
+    split_pair(p[6], p[7], &f.hi.w, &f.lo.w, tag);
+    return f;
+}
+
+// ---------------------------------------------------------------------------------------
+// V pieces of one wave tile, as loaded: piece j of a lane belongs to key 16 (j / 4) + 4 g + j % 4.
+template <typename T, int DH> struct VTile {
+    using G = TreeGeo<T, DH>;
+    static constexpr int NJ = 4 * G::NU;
+    static constexpr int WORDS = G::E * (int)sizeof(T) / 4;     // 32-bit words of a piece: 2 or 4
+    uint32_t w[NJ][G::NBLK][WORDS];
+    uint32_t tail[G::TAIL ? NJ : 1];
+
+    __device__ __forceinline__ void load(int j, const char* row, int c) {
+#pragma unroll
+        for (int b = 0; b < G::NBLK; ++b) {
+            const char* p = row + (b * 16 + c) * (WORDS * 4);
+            if constexpr (WORDS == 4) {
+                const uint4 v = ld16(p);
+                w[j][b][0] = v.x; w[j][b][1] = v.y; w[j][b][2] = v.z; w[j][b][3] = v.w;
+            } else {
+                typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
+                const u32x2_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(p));
+                w[j][b][0] = v.x; w[j][b][1] = v.y;
+            }
+        }
+        if constexpr (G::TAIL != 0) {
+            const char* p = row + (G::NBLK * 16 * G::E + c) * (int)sizeof(T);
+            if constexpr (sizeof(T) == 4) tail[j] = *reinterpret_cast<const uint32_t*>(p);
+            else tail[j] = *reinterpret_cast<const uint16_t*>(p);
+        }
+    }
+    // Key j holds nothing (a slot outside the sample's keys).
+    __device__ __forceinline__ void clear(int j) {
+#pragma unroll
+        for (int b = 0; b < G::NBLK; ++b)
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) w[j][b][i] = 0;
+        if constexpr (G::TAIL != 0) tail[j] = 0;
+    }
+    // Infinities and NaN of key j become zero; true if there was one.
+    __device__ __forceinline__ bool drop_nonfinite(int j) {
+        bool any = false;
+        auto word = [&](uint32_t x) -> uint32_t {
+            if constexpr (sizeof(T) == 4) {
+                const bool bad = (x & 0x7f800000u) == 0x7f800000u;
+                any |= bad;
+                return bad ? 0u : x;
+            } else {
+                constexpr uint32_t e = __is_same(T, bf16_t) ? 0x7f80u : 0x7c00u;
+                const bool lo = (x & e) == e, hi = ((x >> 16) & e) == e;
+                any |= lo | hi;
+                return x & (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu);
+            }
+        };
+#pragma unroll
+        for (int b = 0; b < G::NBLK; ++b)
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) w[j][b][i] = word(w[j][b][i]);
+        if constexpr (G::TAIL != 0) tail[j] = word(tail[j]);
+        return any;
+    }
+    // Left operand of result tile (block b, element e): 8 keys of dim b * 16 E + c * E + e.
+    __device__ __forceinline__ uint4 turned(int b, int e) const {
+        uint32_t o[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            if (b < G::NBLK) o[p] = __builtin_amdgcn_perm(w[2 * p + 1][b][e / 2], w[2 * p][b][e / 2], e % 2 ? 0x07060302 : 0x05040100);
+            else o[p] = __builtin_amdgcn_perm(tail[G::TAIL ? 2 * p + 1 : 0], tail[G::TAIL ? 2 * p : 0], 0x05040100);
+        }
+        return make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    __device__ __forceinline__ float at(int j, int b, int e) const {   // fp32
+        return __builtin_bit_cast(float, b < G::NBLK ? w[j][b][e] : tail[G::TAIL ? j : 0]);
+    }
+};
+
+// Dim of result tile `db`, result row i (0 .. 15).
+template <typename T, int DH> __device__ __forceinline__ int tile_dim(int db, int i) {
+    using G = TreeGeo<T, DH>;
+    if (db < G::NBLK * G::E) return (db / G::E) * 16 * G::E + i * G::E + db % G::E;
+    return G::NBLK * 16 * G::E + i;
+}
+
+template <typename T> __device__ __forceinline__ float load_elem(const T* p);
+template <> __device__ __forceinline__ float load_elem(const uint16_t* p) { return (float)__builtin_bit_cast(_Float16, *p); }
+template <> __device__ __forceinline__ float load_elem(const bf16_t* p) { return bf16_to_float(p->bits); }
+template <> __device__ __forceinline__ float load_elem(const float* p) { return *p; }
+
+// Slots of sample b: [first, length).
+__device__ __forceinline__ void sample_range(const int* first_keys, const int* lengths, int b, int t, int* first, int* length) {
+    const int n = lengths ? min(max(lengths[b], 0), t) : t;
+    *length = n;
+    *first = first_keys ? min(max(first_keys[b], 0), n) : 0;
+}
+
+// Ancestors of node `lane`, itself included, as a bit mask, by one wave: the parent relation is
+// squared six times (64 nodes are at most 63 steps from the root).
+__device__ __forceinline__ uint64_t ancestor_mask(const int* parents, int tokens, int lane) {
+    if (parents == nullptr) return lane == 63 ? ~0ull : (2ull << lane) - 1;
+    int up = lane < tokens ? parents[lane] : -1;
+    if (up < 0 || up >= lane) up = -1;
+    uint32_t lo = lane < 32 ? 1u << lane : 0u, hi = lane < 32 ? 0u : 1u << (lane - 32);
+#pragma unroll
+    for (int s = 0; s < 6; ++s) {
+        const int from = up < 0 ? lane : up;
+        const uint32_t l2 = __shfl((int)lo, from), h2 = __shfl((int)hi, from);
+        const int u2 = __shfl(up, from);
+        lo |= l2;
+        hi |= h2;
+        up = up < 0 ? -1 : u2;
+    }
+    return ((uint64_t)hi << 32) | lo;
+}
+
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+
+// ---------------------------------------------------------------------------------------
+template <typename T, int DH, int RT>
+__global__ void __launch_bounds__(kTreeWaves * 64) ffa_tree_kernel(const TreeParams P) {
+    using G = TreeGeo<T, DH>;
+    constexpr int W = kTreeWaves, NU = G::NU, TK = G::TK, KK = G::KK, NCH = G::NCH, DB = G::DB;
+    constexpr int RS = DH + 4;  // floats of a row in the merge buffer
+    __shared__ float s_acc[W][16 * RS];
+    __shared__ float s_ml[W][RT * 16][2];
+    __shared__ uint64_t s_seen[64];
+    __shared__ unsigned s_bad[2];
+
+    // Row blocks of one piece are 8 workgroups apart: the same XCD, whose L2 then holds the piece.
+    const int span = 8 * P.row_blocks;
+    const int octet = blockIdx.x / span, in = blockIdx.x % span;
+    const int rb = in / 8, piece = octet * 8 + in % 8;
+    const int pairs = P.B * P.H;
+    if (piece >= pairs * P.n_splits) return;
+    const int pair = piece / P.n_splits, split = piece % P.n_splits;
+    const int b = pair / P.H, h = pair % P.H;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, c = lane & 15;
+
+    int first, length;
+    sample_range(P.first_keys, P.lengths, b, P.t, &first, &length);
+    const int count = P.counts ? min(max(P.counts[b], 0), P.tokens) : P.tokens;
+    const bool last = split == P.n_splits - 1;
+    const size_t cache_row = (size_t)DH * sizeof(T);
+    const char* kc = static_cast<const char*>(P.k_cache) + (size_t)pair * P.Lmax * cache_row;
+    const char* vc = static_cast<const char*>(P.v_cache) + (size_t)pair * P.Lmax * cache_row;
+    const char* kn = static_cast<const char*>(P.k) + (b * P.k_stride[0] + h * P.k_stride[1]) * (long long)sizeof(T);
+    const char* vn = static_cast<const char*>(P.v) + (b * P.v_stride[0] + h * P.v_stride[1]) * (long long)sizeof(T);
+    const long long kn_row = P.k_stride[2] * (long long)sizeof(T), vn_row = P.v_stride[2] * (long long)sizeof(T);
+    const int row0 = rb * RT * 16;
+
+    if (tid < 2) s_bad[tid] = 0;
+    if (wave == 0) s_seen[lane] = ancestor_mask(P.parents ? P.parents + (size_t)b * P.tokens : nullptr, P.tokens, lane);
+
+    // Q: chunk kk * 4 + g of row row0 + rt * 16 + c; rows and chunks that do not exist are zero.
+    uint4 qf[RT][KK];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int row = row0 + rt * 16 + c;
+        const int token = row / P.G, gh = row % P.G;
+        const char* qr = static_cast<const char*>(P.q) +
+                         (b * P.q_stride[0] + (long long)(h * P.G + gh) * P.q_stride[1] + token * P.q_stride[2]) * (long long)sizeof(T);
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            const int ch = kk * 4 + g;
+            qf[rt][kk] = make_uint4(0, 0, 0, 0);
+            if (row < P.rows && ch < NCH) qf[rt][kk] = *reinterpret_cast<const uint4*>(qr + ch * 16);
+        }
+    }
+    __syncthreads();
+
+    f32x4_t acc[RT][DB];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        m[rt] = -INFINITY;
+        l[rt] = 0.f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[rt][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    uint4 kf[NU][KK];
+    VTile<T, DH> vt;
+
+    // A chunk that does not exist (Dh = 80) must not hold an infinity against the zero of Q.
+    auto existing = [&](const uint4& x, int kk) {
+        if (NCH % 4 != 0 && kk == KK - 1 && kk * 4 + g >= NCH) return make_uint4(0, 0, 0, 0);
+        return x;
+    };
+    // The loads of a tile of cached keys.  Slots past the sample's end are read from its last slot.
+    auto load_k = [&](int tile) {
+        const int key0 = tile * TK;
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            const int key = min(key0 + u * 16 + c, length - 1);
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+                const int gg = NCH % 4 != 0 && kk == KK - 1 ? min(g, NCH - 1 - kk * 4) : g;
+                const char* base = kc + (size_t)kk * 4 * P.Lmax * 16;
+                kf[u][kk] = existing(ld16(base + ((unsigned)gg * (unsigned)P.Lmax + (unsigned)key) * 16u), kk);
+            }
+        }
+    };
+    auto load_v = [&](int tile) {
+        const int key0 = tile * TK;
+        const char* base = vc + (size_t)key0 * cache_row;
+        const int most = length - 1 - key0;
+#pragma unroll
+        for (int j = 0; j < 4 * NU; ++j) {
+            const int k = (j / 4) * 16 + g * 4 + j % 4;
+            vt.load(j, base + (unsigned)min(k, most) * (unsigned)cache_row, c);
+        }
+    };
+
+    // One tile: scores, weights, products.  seen(row tile, key of the tile) is asked if `masked`.
+    auto tile_step = [&](auto masked, auto seen, int score_key, auto next_k, auto next_v) {
+        constexpr bool MASKED = decltype(masked)::value;
+        f32x4_t s[RT][NU];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                s[rt][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) s[rt][u] = mma_qk(kf[u][kk], qf[rt][kk], s[rt][u], T{});
+            }
+        next_k();
+        PFrag16 pf[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            float x[4 * NU], top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4 * NU; ++j) {
+                x[j] = s[rt][j / 4][j % 4] * P.scale_log2e;
+                if (MASKED && !seen(rt, (j / 4) * 16 + g * 4 + j % 4)) x[j] = -INFINITY;
+                top = fmaxf(top, x[j]);
+            }
+            if (P.ws_scores != nullptr) {
+                const int row = row0 + rt * 16 + c;
+                if (row < P.rows) {
+                    float* to = P.ws_scores + ((size_t)pair * P.rows + row) * P.score_stride + score_key + g * 4;
+#pragma unroll
+                    for (int u = 0; u < NU; ++u)
+                        *reinterpret_cast<float4*>(to + u * 16) = make_float4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
+                }
+            }
+            if (__any(top > m[rt] + kSlack)) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float to = top > m[rt] + kSlack ? top - kLift : m[rt];
+                const float f = to == m[rt] ? 1.f : __builtin_amdgcn_exp2f(m[rt] - to);
+                m[rt] = to;
+                l[rt] *= f;
+#pragma unroll
+                for (int db = 0; db < DB; ++db) acc[rt][db] *= f;
+            }
+            const float ref = m[rt] == -INFINITY ? 0.f : m[rt];
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4 * NU; ++j) {
+                x[j] = __builtin_amdgcn_exp2f(x[j] - ref);
+                sum += x[j];
+            }
+            l[rt] += sum;
+            if constexpr (sizeof(T) == 2) {
+                pf[rt] = split_weights(x, T{});
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[rt][0][j] = x[j];
+            }
+        }
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+            const int blk = db < G::NBLK * G::E ? db / G::E : G::NBLK, e = db < G::NBLK * G::E ? db % G::E : 0;
+            if constexpr (sizeof(T) == 2) {
+                const uint4 a = vt.turned(blk, e);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    acc[rt][db] = mma_qk(a, pf[rt].hi, acc[rt][db], T{});
+                    acc[rt][db] = mma_qk(a, pf[rt].lo, acc[rt][db], T{});
+                }
+            } else {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        acc[rt][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(vt.at(j, blk, e), s[rt][0][j], acc[rt][db], 0, 0, 0);
+            }
+        }
+        next_v();
+    };
+    // ---- cached keys: tiles wave, wave + W, ... of the piece ----
+    {
+        const int lo = max(split * P.tiles_per_split, first / TK);
+        const int hi = min((split + 1) * P.tiles_per_split, (length + TK - 1) / TK);
+        int tile = lo + wave;
+        if (tile < hi) {
+            load_k(tile);
+            load_v(tile);
+        }
+        for (; tile < hi; tile += W) {
+            const int key0 = tile * TK, next = tile + W;
+            auto nk = [&]() { if (next < hi) load_k(next); };
+            auto nv = [&]() { if (next < hi) load_v(next); };
+            if (key0 >= first && key0 + TK <= length) {
+                tile_step(No{}, [](int, int) { return true; }, key0, nk, nv);
+            } else {
+                auto real = [&](int k) { return key0 + k >= first && key0 + k < length; };
+#pragma unroll
+                for (int j = 0; j < 4 * NU; ++j)
+                    if (!real((j / 4) * 16 + g * 4 + j % 4)) vt.clear(j);
+                tile_step(Yes{}, [&](int, int k) { return real(k); }, key0, nk, nv);
+            }
+        }
+    }
+
+    // ---- the new tokens themselves, dealt to the waves from the last: the piece's shorter ends ----
+    if (last) {
+        const int tiles = (count + TK - 1) / TK;
+        for (int d = W - 1 - wave; d < tiles; d += W) {
+            const int node0 = d * TK;
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                const int node = min(node0 + u * 16 + c, count - 1);
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) {
+                    const int ch = min(kk * 4 + g, NCH - 1);
+                    kf[u][kk] = existing(*reinterpret_cast<const uint4*>(kn + node * kn_row + ch * 16), kk);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4 * NU; ++j) {
+                const int node = node0 + (j / 4) * 16 + g * 4 + j % 4;
+                vt.load(j, vn + min(node, count - 1) * vn_row, c);
+                // What is not finite is added at the end, to the rows that see it.
+                if (node >= count) vt.clear(j);
+                else if (vt.drop_nonfinite(j)) atomicOr(&s_bad[node / 32], 1u << (node % 32));
+            }
+            uint64_t mask[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const int row = row0 + rt * 16 + c;
+                mask[rt] = row < P.rows ? s_seen[row / P.G] >> node0 : 0;
+            }
+            tile_step(Yes{}, [&](int rt, int k) { return (bool)((mask[rt] >> k) & 1); }, P.score_stride - 32, [] {}, [] {});
+        }
+    }
+
+    // ---- join the waves ----
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        float sum = l[rt];
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if (g == 0) {
+            s_ml[wave][rt * 16 + c][0] = m[rt];
+            s_ml[wave][rt * 16 + c][1] = sum;
+        }
+    }
+    __syncthreads();
+    const bool whole = P.n_splits == 1;
+    const uint64_t bad = ((uint64_t)s_bad[1] << 32) | s_bad[0];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int mine = rt * 16 + c;
+        float top = s_ml[0][mine][0];
+#pragma unroll
+        for (int w = 1; w < W; ++w) top = fmaxf(top, s_ml[w][mine][0]);
+        const float f = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - top);
+        if (rt > 0) __syncthreads();
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                s_acc[wave][c * RS + tile_dim<T, DH>(db, g * 4 + r)] = m[rt] == -INFINITY ? 0.f : acc[rt][db][r] * f;
+        __syncthreads();
+        // 16 rows x DH outputs, four dims a thread.
+        for (int i = tid; i < 16 * DH / 4; i += W * 64) {
+            const int r = i / (DH / 4), d = (i % (DH / 4)) * 4;
+            const int row = row0 + rt * 16 + r;
+            if (row >= P.rows) continue;
+            const int token = row / P.G;
+            float M = s_ml[0][rt * 16 + r][0];
+#pragma unroll
+            for (int w = 1; w < W; ++w) M = fmaxf(M, s_ml[w][rt * 16 + r][0]);
+            float L = 0.f;
+            f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float mw = s_ml[w][rt * 16 + r][0];
+                if (mw != -INFINITY) L += s_ml[w][rt * 16 + r][1] * __builtin_amdgcn_exp2f(mw - M);
+                o += *reinterpret_cast<const f32x4_t*>(&s_acc[w][r * RS + d]);
+            }
+            if (bad != 0) {
+                for (uint64_t todo = bad & s_seen[token]; todo != 0; todo &= todo - 1) {
+                    const int node = __ffsll((unsigned long long)todo) - 1;
+                    const T* vr = reinterpret_cast<const T*>(vn + node * vn_row) + d;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = load_elem(vr + e);
+                        if (!__builtin_isfinite(x)) o[e] += x;
+                    }
+                }
+            }
+            const size_t slot = ((size_t)pair * P.n_splits + split) * P.rows + row;
+            if ((!whole || P.ws_scores != nullptr) && d == 0) {
+                P.ws_ml[slot * 2] = M;
+                P.ws_ml[slot * 2 + 1] = L;
+            }
+            if (!whole) {
+                *reinterpret_cast<f32x4_t*>(P.ws_acc + slot * DH + d) = o;
+            } else if (token < count) {
+                const int gh = row % P.G;
+                T* to = static_cast<T*>(P.out) + b * P.out_stride[0] + (long long)(h * P.G + gh) * P.out_stride[1] + token * P.out_stride[2];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) store_out(to, d + e, o[e] / L);
+            }
+        }
+    }
+
+    // ---- append the new tokens: no one reads cache slots from `length` on ----
+    if (last && rb == 0) {
+        char* kw = const_cast<char*>(kc);
+        char* vw = const_cast<char*>(vc);
+        for (int i = tid; i < count * NCH; i += W * 64) {
+            const int node = i / NCH, ch = i % NCH, slot = length + node;
+            const uint4 x = *reinterpret_cast<const uint4*>(kn + node * kn_row + ch * 16);
+            const uint4 y = *reinterpret_cast<const uint4*>(vn + node * vn_row + ch * 16);
+            st16(kw + ((size_t)ch * P.Lmax + slot) * 16, x);
+            st16(vw + slot * cache_row + ch * 16, y);
+        }
+    }
+}
+
+// Joins the pieces of a row: out = sum_i O_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).  Four dims a thread.
+template <typename T, int DH>
+__global__ void __launch_bounds__(256) ffa_tree_join_kernel(const TreeParams P) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long line = i / (DH / 4);
+    const int d = (int)(i % (DH / 4)) * 4;
+    if (line >= (long long)P.B * P.H * P.rows) return;
+    const int pair = (int)(line / P.rows), row = (int)(line % P.rows);
+    const int b = pair / P.H, h = pair % P.H, token = row / P.G;
+    if (P.counts && token >= P.counts[b]) return;
+    const size_t slot0 = (size_t)pair * P.n_splits * P.rows + row;
+    float M = -INFINITY;
+    for (int s = 0; s < P.n_splits; ++s) M = fmaxf(M, P.ws_ml[(slot0 + (size_t)s * P.rows) * 2]);
+    float L = 0.f;
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < P.n_splits; ++s) {
+        const size_t slot = slot0 + (size_t)s * P.rows;
+        const float ms = P.ws_ml[slot * 2];
+        if (ms == -INFINITY) continue;
+        const float f = __builtin_amdgcn_exp2f(ms - M);
+        L += P.ws_ml[slot * 2 + 1] * f;
+        o += *reinterpret_cast<const f32x4_t*>(P.ws_acc + slot * DH + d) * f;
+    }
+    T* to = static_cast<T*>(P.out) + b * P.out_stride[0] + (long long)(h * P.G + row % P.G) * P.out_stride[1] + token * P.out_stride[2];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) store_out(to, d + e, o[e] / L);
+}
+
+// Weight-summing step, after the scores and the pieces' (m, l) are known: every key's weight.
+static __global__ void __launch_bounds__(256) ffa_tree_weights_kernel(const TreeParams P, int blocks) {
+    const int pair = blockIdx.x / blocks, b = pair / P.H;
+    int first, length;
+    sample_range(P.first_keys, P.lengths, b, P.t, &first, &length);
+    const int j = (blockIdx.x % blocks) * 256 + threadIdx.x;
+    if (j > length) return;
+    float w = 0.f;
+    for (int row = 0; row < P.rows; ++row) {
+        const size_t slot0 = (size_t)pair * P.n_splits * P.rows + row;
+        float M = -INFINITY, L = 0.f;
+        for (int s = 0; s < P.n_splits; ++s) M = fmaxf(M, P.ws_ml[(slot0 + (size_t)s * P.rows) * 2]);
+        for (int s = 0; s < P.n_splits; ++s) {
+            const float ms = P.ws_ml[(slot0 + (size_t)s * P.rows) * 2];
+            if (ms != -INFINITY) L += P.ws_ml[(slot0 + (size_t)s * P.rows) * 2 + 1] * __builtin_amdgcn_exp2f(ms - M);
+        }
+        const float* x = P.ws_scores + ((size_t)pair * P.rows + row) * P.score_stride;
+        if (j >= first) w += __builtin_amdgcn_exp2f(x[j == length ? P.score_stride - 32 : j] - M) / L;
+    }
+    float* to = P.key_weights + (size_t)pair * P.Lmax + j;
+    if (j == length) *to = w;
+    else if (j >= first) *to += w;
+}
+
+// ---------------------------------------------------------------------------------------
+template <typename T, int DH> int launch_tree_dh(const TreeParams& P, int row_tiles, hipStream_t st) {
+    const int pieces = P.B * P.H * P.n_splits;
+    const dim3 grid((unsigned)((pieces + 7) / 8 * 8 * P.row_blocks)), block(kTreeWaves * 64);
+    switch (row_tiles) {
+        case 1: hipLaunchKernelGGL((ffa_tree_kernel<T, DH, 1>), grid, block, 0, st, P); break;
+        case 2: hipLaunchKernelGGL((ffa_tree_kernel<T, DH, 2>), grid, block, 0, st, P); break;
+        default:
+            if constexpr (DH != 256) {
+                if (row_tiles == 3) hipLaunchKernelGGL((ffa_tree_kernel<T, DH, 3>), grid, block, 0, st, P);
+                else hipLaunchKernelGGL((ffa_tree_kernel<T, DH, 4>), grid, block, 0, st, P);
+                break;
+            }
+            return FFA_ERR_PLAN;
+    }
+    if (hipGetLastError() != hipSuccess) return FFA_ERR_LAUNCH;
+    if (P.n_splits > 1) {
+        const long long threads = (long long)P.B * P.H * P.rows * (DH / 4);
+        hipLaunchKernelGGL((ffa_tree_join_kernel<T, DH>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, P);
+        if (hipGetLastError() != hipSuccess) return FFA_ERR_LAUNCH;
+    }
+    if (P.ws_scores != nullptr) {
+        const int blocks = (P.t + 1 + 255) / 256;
+        hipLaunchKernelGGL(ffa_tree_weights_kernel, dim3((unsigned)(P.B * P.H * blocks)), dim3(256), 0, st, P, blocks);
+        if (hipGetLastError() != hipSuccess) return FFA_ERR_LAUNCH;
+    }
+    return FFA_OK;
+}
+
+template <typename T> int launch_tree_type(const TreeParams& P, int head_dim, int row_tiles, void* stream) {
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    switch (head_dim) {
+        case 64: return launch_tree_dh<T, 64>(P, row_tiles, st);
+        case 80: return launch_tree_dh<T, 80>(P, row_tiles, st);
+        case 128: return launch_tree_dh<T, 128>(P, row_tiles, st);
+        case 256: return launch_tree_dh<T, 256>(P, row_tiles, st);
+        default: return FFA_ERR_HEAD_DIM;
+    }
+}
+
+}  // namespace ffa

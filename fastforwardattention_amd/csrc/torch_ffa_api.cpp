@@ -20,6 +20,7 @@
 
 #include <tuple>
 #include <utility>
+#include <vector>
 
 #include "ffa_c_api.h"
 
@@ -78,6 +79,221 @@ torch::Tensor token_input(const torch::Tensor& x, const torch::Tensor& like, int
     TORCH_CHECK(x.numel() == numel, "ff_attention: ", name, " must hold B*H*Dh = ", numel,
                 " elements, got ", x.numel());
     return x.contiguous();  // storage order [B,H,Dh]; no copy when already contiguous
+}
+
+// A contiguous tensor may start anywhere in its storage; the kernels read 16 bytes at a time.
+torch::Tensor aligned_input(const torch::Tensor& x) {
+    return (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) == 0 ? x : x.clone();
+}
+
+// ---------------------------------------------------------------------------------------
+// Operators next to the decode step.  None of them has a counterpart in the reference; they work on
+// caches of the layouts get_cache() returns and keep nothing between calls: workspaces come from
+// torch's allocator, which hands them out in stream order.
+using OptTensor = c10::optional<torch::Tensor>;
+using CachePair = std::pair<torch::Tensor, torch::Tensor>;
+using CacheTriple = std::tuple<torch::Tensor, torch::Tensor, torch::Tensor>;
+
+CacheDims checked_caches(const torch::Tensor& k_cache, const torch::Tensor& v_cache) {
+    TORCH_CHECK(k_cache.is_cuda() && v_cache.is_cuda() && k_cache.device() == v_cache.device() &&
+                    k_cache.scalar_type() == v_cache.scalar_type(),
+                "ff_attention: caches must be GPU tensors of one dtype on one device");
+    return dims_of(k_cache, v_cache);
+}
+
+// An int32 tensor of `shape` on the caches' device; empty = not given.
+torch::Tensor int_input(const OptTensor& x, const torch::Tensor& like, at::IntArrayRef shape, const char* name) {
+    if (!x.has_value()) return torch::Tensor();
+    TORCH_CHECK(x->device() == like.device() && x->scalar_type() == torch::kInt && x->sizes() == shape,
+                "ff_attention: ", name, " must be an int32 tensor of shape ", shape, " on the caches' device");
+    return x->contiguous();
+}
+const int* int_ptr(const torch::Tensor& x) { return x.defined() ? x.data_ptr<int>() : nullptr; }
+
+// [B, heads, n, Dh] in any order of its first three dimensions; copied only if a row is not
+// contiguous or not made of aligned 16-byte pieces.
+torch::Tensor group_input(const torch::Tensor& x, const torch::Tensor& like, const char* name) {
+    TORCH_CHECK(x.device() == like.device() && x.scalar_type() == like.scalar_type(), "ff_attention: ", name,
+                " must have the caches' dtype and device");
+    const int64_t unit = 16 / x.element_size();
+    bool fits = x.stride(3) == 1 && (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) == 0;
+    for (int i = 0; i < 3; ++i) fits = fits && x.stride(i) % unit == 0;
+    return fits ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+torch::Tensor scratch(size_t bytes, const torch::Tensor& like) {
+    return torch::empty({(int64_t)bytes}, torch::TensorOptions().dtype(torch::kUInt8).device(like.device()));
+}
+
+// Attention of a group of n new tokens a sample: q [B,Hq,n,Dh], k, v [B,H,n,Dh] -> [B,Hq,n,Dh].
+torch::Tensor attention_tree(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor k_cache,
+                             torch::Tensor v_cache, float softmax_scale, int t, OptTensor parents, OptTensor first_keys,
+                             OptTensor lengths, OptTensor counts) {
+    const CacheDims d = checked_caches(k_cache, v_cache);
+    TORCH_CHECK(q.dim() == 4 && q.size(0) == d.B && q.size(3) == d.Dh && q.size(1) > 0 && q.size(1) % d.H == 0,
+                "ff_attention: q must be [B, Hq, n, Dh] with Hq a multiple of the caches' heads, got ", q.sizes());
+    const int64_t n = q.size(2);
+    TORCH_CHECK(n >= 1 && n <= FFA_MAX_TREE_TOKENS, "ff_attention: a group holds 1 to ", FFA_MAX_TREE_TOKENS,
+                " new tokens a sample, got ", n);
+    TORCH_CHECK(k.sizes() == at::IntArrayRef({d.B, d.H, n, d.Dh}) && v.sizes() == k.sizes(),
+                "ff_attention: k and v must be [B, H, n, Dh] with q's n, got ", k.sizes(), " and ", v.sizes());
+    TORCH_CHECK(t >= 0 && n <= d.Lmax && t <= d.Lmax - n, "ff_attention: ", n, " tokens at timestep ", t,
+                " do not fit the cache [0, ", d.Lmax, ")");
+    const int precision = precision_of(k_cache);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
+    q = group_input(q, k_cache, "q");
+    k = group_input(k, k_cache, "k");
+    v = group_input(v, k_cache, "v");
+    const torch::Tensor par = int_input(parents, k_cache, {d.B, n}, "parents");
+    const torch::Tensor fk = int_input(first_keys, k_cache, {d.B}, "first_keys");
+    const torch::Tensor len = int_input(lengths, k_cache, {d.B}, "lengths");
+    const torch::Tensor cnt = int_input(counts, k_cache, {d.B}, "counts");
+    // Token-major in memory, so that [B, n, Hq * Dh] is a view; rows past a sample's count are zero.
+    const int64_t Hq = q.size(1);
+    torch::Tensor out = (cnt.defined() ? torch::zeros({d.B, n, Hq, d.Dh}, q.options())
+                                       : torch::empty({d.B, n, Hq, d.Dh}, q.options())).transpose(1, 2);
+    ffa_tree_tokens tt = {};
+    tt.tokens = (int)n;
+    tt.q_head_num = (int)Hq;
+    tt.parents = int_ptr(par);
+    tt.first_keys = int_ptr(fk);
+    tt.lengths = int_ptr(len);
+    tt.counts = int_ptr(cnt);
+    for (int i = 0; i < 3; ++i) {
+        tt.q_stride[i] = q.stride(i);
+        tt.k_stride[i] = k.stride(i);
+        tt.v_stride[i] = v.stride(i);
+        tt.out_stride[i] = out.stride(i);
+    }
+    const size_t bytes = ffa_tree_workspace_bytes(precision, d.B, d.H, (int)Hq, d.Dh, (int)n, t);
+    const torch::Tensor ws = scratch(bytes, k_cache);
+    check_status(ffa_attention_tree(precision, d.B, d.H, d.Dh, d.Lmax, softmax_scale, t, &tt, q.data_ptr(), k.data_ptr(),
+                                    v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
+                                    bytes ? ws.data_ptr() : nullptr, bytes, stream_of(k_cache)),
+                 "attention_tree");
+    return out;
+}
+
+// The one-token step that adds its softmax weights to key_weights: q [B,Hq,Dh] -> [B,Hq,Dh].
+torch::Tensor attention_weights(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor k_cache,
+                                torch::Tensor v_cache, float softmax_scale, int t, torch::Tensor key_weights,
+                                OptTensor first_keys, OptTensor lengths) {
+    const CacheDims d = checked_caches(k_cache, v_cache);
+    const int64_t per = (int64_t)d.B * d.Dh;
+    TORCH_CHECK(q.numel() > 0 && q.numel() % (per * d.H) == 0,
+                "ff_attention: q must hold B*Hq*Dh elements with Hq a multiple of the caches' heads, got ", q.sizes());
+    const int64_t Hq = q.numel() / per;
+    TORCH_CHECK(t >= 0 && t < d.Lmax, "ff_attention: timestep ", t, " outside the cache [0, ", d.Lmax, ")");
+    TORCH_CHECK(key_weights.device() == k_cache.device() && key_weights.scalar_type() == torch::kFloat &&
+                    key_weights.is_contiguous() && key_weights.sizes() == at::IntArrayRef({d.B, d.H, d.Lmax}),
+                "ff_attention: key_weights must be a contiguous float32 tensor [B, H, max_len] on the caches' device");
+    const int precision = precision_of(k_cache);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
+    q = aligned_input(token_input(q, k_cache, per * Hq, "q"));
+    k = aligned_input(token_input(k, k_cache, per * d.H, "k"));
+    v = aligned_input(token_input(v, k_cache, per * d.H, "v"));
+    const torch::Tensor fk = int_input(first_keys, k_cache, {d.B}, "first_keys");
+    const torch::Tensor len = int_input(lengths, k_cache, {d.B}, "lengths");
+    torch::Tensor out = torch::empty({d.B, Hq, d.Dh}, q.options());
+    const size_t bytes = ffa_weights_workspace_bytes(precision, d.B, d.H, (int)Hq, d.Dh, t);
+    const torch::Tensor ws = scratch(bytes, k_cache);
+    check_status(ffa_attention_weights(precision, d.B, d.H, (int)Hq, d.Dh, d.Lmax, softmax_scale, t, q.data_ptr(),
+                                       k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
+                                       key_weights.data_ptr<float>(), int_ptr(fk), int_ptr(len),
+                                       bytes ? ws.data_ptr() : nullptr, bytes, stream_of(k_cache)),
+                 "attention_weights");
+    return out;
+}
+
+// Caches of one shape, type and device, one a layer.
+CacheDims layer_caches(const std::vector<CachePair>& caches) {
+    TORCH_CHECK(!caches.empty(), "ff_attention: no caches");
+    const CacheDims d = checked_caches(caches[0].first, caches[0].second);
+    for (const auto& c : caches) {
+        TORCH_CHECK(c.first.sizes() == caches[0].first.sizes() && c.first.scalar_type() == caches[0].first.scalar_type() &&
+                        c.first.device() == caches[0].first.device(),
+                    "ff_attention: the caches of a call must share shape, dtype and device");
+        checked_caches(c.first, c.second);
+    }
+    return d;
+}
+
+// Moves the accepted path of every sample's tree behind its length, in all layers' caches.
+void commit_tree(const std::vector<CachePair>& caches, int t, torch::Tensor path, torch::Tensor accepted,
+                 OptTensor lengths) {
+    const CacheDims d = layer_caches(caches);
+    const torch::Tensor& like = caches[0].first;
+    TORCH_CHECK(path.dim() == 2 && path.size(1) >= 1 && path.size(1) <= FFA_MAX_TREE_TOKENS,
+                "ff_attention: path must be [B, 1 .. ", FFA_MAX_TREE_TOKENS, "], got ", path.sizes());
+    const int64_t m = path.size(1);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(like.device());
+    path = int_input(path, like, {d.B, m}, "path");
+    accepted = int_input(accepted, like, {d.B}, "accepted");
+    const torch::Tensor len = int_input(lengths, like, {d.B}, "lengths");
+    std::vector<void*> k, v;
+    for (const auto& c : caches) {
+        k.push_back(c.first.data_ptr());
+        v.push_back(c.second.data_ptr());
+    }
+    check_status(ffa_commit_tree(precision_of(like), (int)caches.size(), k.data(), v.data(), d.B, d.H, d.Dh, d.Lmax, t,
+                                 path.data_ptr<int>(), (int)m, accepted.data_ptr<int>(), int_ptr(len), stream_of(like)),
+                 "commit_tree");
+}
+
+// Keeps the last `recent` and the heaviest of the others, `keep` slots a pair in all; returns the
+// old slots kept, int32 [caches, B, H, keep].
+torch::Tensor evict(const std::vector<CachePair>& caches, const std::vector<torch::Tensor>& key_weights, int t, int keep,
+                    int recent, OptTensor first_keys, OptTensor lengths, c10::optional<std::vector<CacheTriple>> into) {
+    const CacheDims d = layer_caches(caches);
+    const torch::Tensor& like = caches[0].first;
+    TORCH_CHECK(key_weights.size() == caches.size() && (!into.has_value() || into->size() == caches.size()),
+                "ff_attention: evict needs one tensor of weights, and one target if any, for each cache");
+    std::vector<CachePair> to;
+    std::vector<torch::Tensor> w_to;
+    if (into.has_value()) {
+        for (const auto& x : *into) {
+            to.emplace_back(std::get<0>(x), std::get<1>(x));
+            w_to.push_back(std::get<2>(x));
+        }
+    } else {
+        to = caches;
+        w_to = key_weights;
+    }
+    const CacheDims e = layer_caches(to);
+    TORCH_CHECK(e.B == d.B && e.H == d.H && e.Dh == d.Dh && to[0].first.scalar_type() == like.scalar_type() &&
+                    to[0].first.device() == like.device(),
+                "ff_attention: a target differs from its cache in more than its length");
+    auto check_weights = [&](const torch::Tensor& w, int len) {
+        TORCH_CHECK(w.device() == like.device() && w.scalar_type() == torch::kFloat && w.is_contiguous() &&
+                        w.sizes() == at::IntArrayRef({d.B, d.H, len}),
+                    "ff_attention: weights must be contiguous float32 tensors [B, H, max_len] on the caches' device");
+    };
+    for (const auto& w : key_weights) check_weights(w, d.Lmax);
+    for (const auto& w : w_to) check_weights(w, e.Lmax);
+    TORCH_CHECK(t >= 0 && t <= d.Lmax, "ff_attention: ", t, " slots in a cache of ", d.Lmax);
+    TORCH_CHECK(keep >= 1 && keep <= e.Lmax && recent >= 0 && recent <= keep, "ff_attention: evict wants 1 <= keep <= ",
+                e.Lmax, " (the target's slots) and 0 <= recent <= keep, got keep ", keep, ", recent ", recent);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(like.device());
+    const torch::Tensor fk = int_input(first_keys, like, {d.B}, "first_keys");
+    const torch::Tensor len = int_input(lengths, like, {d.B}, "lengths");
+    std::vector<const void*> k, v;
+    std::vector<void*> k2, v2;
+    std::vector<const float*> w;
+    std::vector<float*> w2;
+    for (size_t i = 0; i < caches.size(); ++i) {
+        k.push_back(caches[i].first.data_ptr());
+        v.push_back(caches[i].second.data_ptr());
+        w.push_back(key_weights[i].data_ptr<float>());
+        k2.push_back(to[i].first.data_ptr());
+        v2.push_back(to[i].second.data_ptr());
+        w2.push_back(w_to[i].data_ptr<float>());
+    }
+    torch::Tensor kept = torch::empty({(int64_t)caches.size(), d.B, d.H, keep}, like.options().dtype(torch::kInt));
+    check_status(ffa_evict(precision_of(like), (int)caches.size(), k.data(), v.data(), w.data(), k2.data(), v2.data(),
+                           w2.data(), d.B, d.H, d.Dh, d.Lmax, e.Lmax, t, keep, recent, int_ptr(fk), int_ptr(len),
+                           kept.data_ptr<int>(), stream_of(like)),
+                 "evict");
+    return kept;
 }
 
 }  // namespace
@@ -301,5 +517,29 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
              py::arg("cache_indir") = py::none(), py::arg("beam_width") = 1)
         .def("attention_diag", &FastForwardAttn::attention_diag,
              "Attention forward plus (kept_count, skip_mask) of the pruning rule")
+        .def_static("attention_tree", &attention_tree,
+                    "Attention of a group of up to 64 new tokens a sample (a drafted tree, or a chain) over the caches "
+                    "and the tokens' own ancestors; appends them.  q [B,Hq,n,Dh], k, v [B,H,n,Dh] -> [B,Hq,n,Dh]",
+                    py::arg("q"), py::arg("k"), py::arg("v"), py::arg("k_cache"), py::arg("v_cache"),
+                    py::arg("softmax_scale"), py::arg("curr_timestep"), py::arg("parents") = py::none(),
+                    py::arg("first_keys") = py::none(), py::arg("lengths") = py::none(), py::arg("counts") = py::none())
+        .def_static("commit_tree", &commit_tree,
+                    "Moves the accepted path (path int32 [B,m], accepted int32 [B]) behind each sample's length in "
+                    "every (k_cache, v_cache) of the list",
+                    py::arg("caches"), py::arg("curr_timestep"), py::arg("path"), py::arg("accepted"),
+                    py::arg("lengths") = py::none())
+        .def_static("attention_weights", &attention_weights,
+                    "Attention forward of one token that adds the softmax weight every key receives to key_weights "
+                    "(float32 [B,H,max_len])",
+                    py::arg("q"), py::arg("k"), py::arg("v"), py::arg("k_cache"), py::arg("v_cache"),
+                    py::arg("softmax_scale"), py::arg("curr_timestep"), py::arg("key_weights"),
+                    py::arg("first_keys") = py::none(), py::arg("lengths") = py::none())
+        .def_static("evict", &evict,
+                    "Keeps, for every head, the last `recent` slots and the heaviest others, `keep` in all, in slot order "
+                    "at the front of the caches (or of `into`, a list of (k_cache, v_cache, key_weights)); returns the "
+                    "old slots kept, int32 [caches,B,H,keep]",
+                    py::arg("caches"), py::arg("key_weights"), py::arg("curr_timestep"), py::arg("keep"),
+                    py::arg("recent"), py::arg("first_keys") = py::none(), py::arg("lengths") = py::none(),
+                    py::arg("into") = py::none())
         .def("launch_plan", &FastForwardAttn::launch_plan, "Launch plan for (t, p)");
 }

@@ -50,8 +50,15 @@ typedef enum ffa_status {
                                 /* than FFA_STATIC_SCRATCH_BYTES                             */
     FFA_ERR_TRANSFORM = 14,     /* rotary_embedding_dim odd, negative or > head_dim, or a    */
                                 /* bias pointer not 16-byte aligned                          */
-    FFA_ERR_BEAM = 15           /* beam indirection: NULL or misaligned table, beam_width    */
+    FFA_ERR_BEAM = 15,          /* beam indirection: NULL or misaligned table, beam_width    */
                                 /* < 1 or not a divisor of batch_size, or a group too large   */
+    FFA_ERR_TREE = 16,          /* drafted tokens: count outside [1, FFA_MAX_TREE_TOKENS], no */
+                                /* room for them behind t, query heads no multiple of the     */
+                                /* cache's heads, or a stride that is no multiple of 16 bytes */
+    FFA_ERR_EVICT = 17,         /* eviction: keep < 1 or past the target, recent outside      */
+                                /* [0, keep]                                                  */
+    FFA_ERR_OVERLAP = 18        /* eviction: a target overlaps another buffer of the call and */
+                                /* is not exactly its own source                              */
 } ffa_status;
 
 /* precision codes: the same integers the reference passes to get_launch_params
@@ -290,6 +297,106 @@ int ffa_attention_static_scratch(int precision, int batch_size, int head_num, in
 int ffa_load_floor(int precision, int batch_size, int head_num, int head_dim, int max_seq_len, int t,
                    const void* k_cache, const void* v_cache, const int* seq_lengths,
                    int right_or_no_padding, const ffa_launch_plan* plan, void* sink, void* stream);
+
+/*
+ * Operators on the same caches that the reference does not have.  Device arrays of int32 that
+ * describe the samples, each of which may be NULL:
+ *   first_keys [B]  first real slot of a left-padded sample (NULL: 0), clamped to [0, length];
+ *   lengths    [B]  slots that sample b holds (NULL: t), clamped to [0, t].
+ * Their values are read on the device and cannot be refused on the host; every value, also a
+ * wrong one, is brought into range first, so that no access leaves the buffers.
+ */
+
+/*
+ * Attention of a group of new tokens a sample -- the nodes of a drafted tree, or a chain (a
+ * chunk of a prompt, a guess) -- over the cached keys and the node's own ancestors:
+ *   out[b,hq,i] = sum over j of softmax_j(softmax_scale <q[b,hq,i], k_j>) v_j,
+ *   j = cached slots first .. length - 1 and node i with its ancestors.
+ * Node i of sample b is appended at cache slot length + i.  Sums and softmax statistics are fp32;
+ * in 16-bit types the weights enter the matrix products as a sum of two 16-bit numbers, good to
+ * 20 (fp16) or 14 (bf16) bits.
+ *   tokens      nodes a sample, 1 .. FFA_MAX_TREE_TOKENS; t + tokens <= max_seq_len;
+ *   q_head_num  a multiple G * head_num of the cache's heads: query head hq reads head hq / G;
+ *   parents     [B, tokens]: the node's parent, a node before it; any value outside [0, i) makes
+ *               node i a child of the last cached token.  NULL: a chain;
+ *   counts      [B]: sample b has only this many nodes (clamped to [0, tokens]); rows of `out`
+ *               and cache slots of the others stay as they were.  NULL: all;
+ *   *_stride    element strides of (sample, head, token) of q, k, v and out; each row of
+ *               head_dim elements is contiguous, and strides are multiples of 16 bytes.
+ * A slot that no node may see (padding, slots from length on, nodes that are no ancestors) has
+ * no influence whatever it holds, infinities and NaN included.
+ * workspace: ffa_tree_workspace_bytes() for the same arguments (a step with the same arguments and
+ * a smaller t needs no more); it holds nothing between calls and needs no initialisation; calls that
+ * may overlap need one each.
+ */
+#define FFA_MAX_TREE_TOKENS 64
+typedef struct ffa_tree_tokens {
+    int32_t tokens;
+    int32_t q_head_num;
+    const int32_t* parents;
+    const int32_t* first_keys;
+    const int32_t* lengths;
+    const int32_t* counts;
+    int64_t q_stride[3];
+    int64_t k_stride[3];
+    int64_t v_stride[3];
+    int64_t out_stride[3];
+} ffa_tree_tokens;
+
+size_t ffa_tree_workspace_bytes(int precision, int batch_size, int head_num, int q_head_num, int head_dim,
+                                int tokens, int t);
+int ffa_attention_tree(int precision, int batch_size, int head_num, int head_dim, int max_seq_len,
+                       float softmax_scale, int t, const ffa_tree_tokens* tokens, const void* q,
+                       const void* k, const void* v, void* k_cache, void* v_cache, void* out,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * After verification: the accepted path of each sample's tree moves to the slots behind the
+ * sample's length, K and V, in n_caches caches of one shape (one a layer) in one call:
+ *   for j < accepted[b]:  slot length + j  <-  the old slot length + path[b, j].
+ * path [B, path_len] holds node numbers as attention_tree counts them, root first (so each is
+ * larger than the one before); accepted [B] is clamped to [0, path_len], and a slot to the cache.
+ * All old slots of a sample are read before any is written, so that every path is a gather.
+ * path_len 1 .. FFA_MAX_TREE_TOKENS; k_caches and v_caches are HOST arrays of device pointers.
+ */
+int ffa_commit_tree(int precision, int n_caches, void* const* k_caches, void* const* v_caches,
+                    int batch_size, int head_num, int head_dim, int max_seq_len, int t,
+                    const int32_t* path, int path_len, const int32_t* accepted,
+                    const int32_t* lengths, void* stream);
+
+/*
+ * The decode step of one token (q, k, v, out contiguous [B, heads, Dh]) that also sums the
+ * attention a key receives, which ffa_evict goes by:
+ *   key_weights [B, H, max_seq_len] fp32: for first <= j < length, += the softmax weight of key j
+ *   summed over the G query heads of head h; at slot length, the new token's own weight is stored.
+ * Other slots are not touched.  Arguments and workspace as ffa_attention_tree.
+ */
+size_t ffa_weights_workspace_bytes(int precision, int batch_size, int head_num, int q_head_num,
+                                   int head_dim, int t);
+int ffa_attention_weights(int precision, int batch_size, int head_num, int q_head_num, int head_dim,
+                          int max_seq_len, float softmax_scale, int t, const void* q, const void* k,
+                          const void* v, void* k_cache, void* v_cache, void* out, float* key_weights,
+                          const int32_t* first_keys, const int32_t* lengths, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/*
+ * Eviction by accumulated attention weight, in n_caches caches of one shape in one call.  Of the
+ * `length` slots of a (sample, head) pair `keep` stay: the last `recent`, and of those before them
+ * the keep - recent with the largest key_weights -- padding slots (below first) rank behind all
+ * others, equal weights go to the lowest slot, NaN ranks as the smallest weight.  What stays moves,
+ * in slot order, to slots 0 .. keep - 1 of the target, K, V and weight; a pair with no more than
+ * `keep` slots keeps all.  Target slots behind are not touched.  Afterwards sample b holds
+ * min(length, keep) slots, and its padding ends at max(0, first - max(0, length - keep)).
+ *   *_src, *_dst  HOST arrays of device pointers; a target is its own source (in place, same
+ *                 max_seq_len) or overlaps no other buffer of the call, each of k, v and w by itself;
+ *   w_src, w_dst  key_weights [B, H, src_max_seq_len] / [B, H, dst_max_seq_len];
+ *   kept          device int32 [n_caches, B, H, keep]: the old slot of each kept one, -1 behind.
+ */
+int ffa_evict(int precision, int n_caches, const void* const* k_src, const void* const* v_src,
+              const float* const* w_src, void* const* k_dst, void* const* v_dst, float* const* w_dst,
+              int batch_size, int head_num, int head_dim, int src_max_seq_len, int dst_max_seq_len,
+              int t, int keep, int recent, const int32_t* first_keys, const int32_t* lengths,
+              int32_t* kept, void* stream);
 
 #ifdef __cplusplus
 }
