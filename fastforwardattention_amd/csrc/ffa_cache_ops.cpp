@@ -80,6 +80,18 @@ int run_tree(int precision, int head_dim, TreeParams& P, void* workspace, size_t
     return launch_tree(precision, head_dim, P, plan, stream);
 }
 
+// A positive factor for the kernel, so that the largest product is the largest score and a masked
+// -inf stays -inf.  A scale of zero (or one that vanishes in fp32) makes all scores 0: Q is taken as 0.
+void set_scale(TreeParams& P, float softmax_scale) {
+    const float c = softmax_scale * 1.4426950408889634f;
+    P.q_sign = c < 0.f ? -1 : 1;
+    P.scale_log2e = c < 0.f ? -c : c;
+    if (P.scale_log2e < 1.17549435e-38f) {
+        P.q_sign = 0;
+        P.scale_log2e = 1.f;
+    }
+}
+
 size_t tree_workspace(int precision, int B, int H, int Hq, int Dh, int tokens, int t, bool scores) {
     if (check_cache_shape(precision, B, H, Dh, 1) != FFA_OK || Hq <= 0 || Hq % H != 0 || tokens < 1 ||
         tokens > FFA_MAX_TREE_TOKENS || t < 0)
@@ -153,7 +165,7 @@ int ffa_attention_tree(int precision, int batch_size, int head_num, int head_dim
     }
     P.B = batch_size; P.H = head_num; P.G = Hq / head_num; P.tokens = n; P.rows = P.G * n;
     P.Lmax = max_seq_len; P.t = t;
-    P.scale_log2e = softmax_scale * 1.4426950408889634f;
+    set_scale(P, softmax_scale);
     return run_tree(precision, head_dim, P, workspace, workspace_bytes, stream);
 }
 
@@ -183,7 +195,7 @@ int ffa_attention_weights(int precision, int batch_size, int head_num, int q_hea
     }
     P.B = batch_size; P.H = head_num; P.G = q_head_num / head_num; P.tokens = 1; P.rows = P.G;
     P.Lmax = max_seq_len; P.t = t;
-    P.scale_log2e = softmax_scale * 1.4426950408889634f;
+    set_scale(P, softmax_scale);
     return run_tree(precision, head_dim, P, workspace, workspace_bytes, stream);
 }
 

@@ -36,7 +36,8 @@ struct TreeParams {
     float* key_weights;  // weight-summing step: [pairs, Lmax], else nullptr
     int score_stride;
     int B, H, G, tokens, rows, Lmax, t;
-    float scale_log2e;
+    float scale_log2e;  // |softmax_scale| * log2(e), never zero
+    int q_sign;         // sign of softmax_scale: Q enters with it
     int n_splits, tiles_per_split, row_blocks;
 };
 

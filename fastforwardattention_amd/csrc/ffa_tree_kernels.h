@@ -69,21 +69,25 @@ __device__ __forceinline__ f32x4_t mma_qk(const uint4& k, const uint4& q, f32x4_
 // The weights of one row tile as right operands.  16-bit types: P = hi + lo, hi rounded towards
 // zero, so that the weights are off by 2^-20 (fp16) or 2^-14 (bf16) at most and the result is as
 // good as with fp32 weights after its own rounding to 11 or 8 bits.  lo is kept above zero: 0 * V would turn an infinite
-// V into NaN.  (A NaN weight is NaN in hi; fmaxf makes it tiny in lo.)
+// V into NaN.  (A NaN weight is NaN in hi, whatever lo is.)
 struct PFrag16 { uint4 hi, lo; };
+typedef __fp16 fp16x2_t __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint32_t* lo, uint16_t) {
-    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    const half2_t h = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(a, b));
     *hi = __builtin_bit_cast(uint32_t, h);
-    constexpr float tiny = 5.9604644775390625e-8f;  // 2^-24, the smallest fp16
-    *lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaxf(a - (float)h[0], tiny), fmaxf(b - (float)h[1], tiny)));
+    const half2_t rest = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float)h[0], -1.f, a), fmaf((float)h[1], -1.f, b)));
+    const half2_t tiny = __builtin_bit_cast(half2_t, 0x00010001u);  // 2^-24, the smallest fp16
+    *lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(rest, tiny));
 }
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint32_t* lo, bf16_t) {
     const uint32_t ua = __builtin_bit_cast(uint32_t, a), ub = __builtin_bit_cast(uint32_t, b);
     *hi = __builtin_amdgcn_perm(ub, ua, 0x07060302);
-    constexpr float tiny = 5.9604644775390625e-8f;
-    const float la = fmaxf(a - __builtin_bit_cast(float, ua & 0xffff0000u), tiny);
-    const float lb = fmaxf(b - __builtin_bit_cast(float, ub & 0xffff0000u), tiny);
-    *lo = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, lb), __builtin_bit_cast(uint32_t, la), 0x07060302);
+    const float la = a - __builtin_bit_cast(float, ua & 0xffff0000u), lb = b - __builtin_bit_cast(float, ub & 0xffff0000u);
+    const uint32_t rest = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, lb), __builtin_bit_cast(uint32_t, la), 0x07060302);
+    // The rest is not negative: its bit pattern orders as it does.  0x3380 is 2^-24.
+    const u16x2_t tiny = {0x3380, 0x3380};
+    *lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, rest), tiny));
 }
 
 template <typename T> __device__ __forceinline__ PFrag16 split_weights(const float (&p)[8], T tag) {
@@ -104,10 +108,10 @@ template <typename T, int DH> struct VTile {
     uint32_t w[NJ][G::NBLK][WORDS];
     uint32_t tail[G::TAIL ? NJ : 1];
 
-    __device__ __forceinline__ void load(int j, const char* row, int c) {
+    __device__ __forceinline__ void load(int j, const char* row, unsigned lane_row, int c) {
 #pragma unroll
         for (int b = 0; b < G::NBLK; ++b) {
-            const char* p = row + (b * 16 + c) * (WORDS * 4);
+            const char* p = row + b * 16 * WORDS * 4 + (lane_row + (unsigned)c * (WORDS * 4));
             if constexpr (WORDS == 4) {
                 const uint4 v = ld16(p);
                 w[j][b][0] = v.x; w[j][b][1] = v.y; w[j][b][2] = v.z; w[j][b][3] = v.w;
@@ -118,7 +122,7 @@ template <typename T, int DH> struct VTile {
             }
         }
         if constexpr (G::TAIL != 0) {
-            const char* p = row + (G::NBLK * 16 * G::E + c) * (int)sizeof(T);
+            const char* p = row + G::NBLK * 16 * G::E * (int)sizeof(T) + (lane_row + (unsigned)c * (unsigned)sizeof(T));
             if constexpr (sizeof(T) == 4) tail[j] = *reinterpret_cast<const uint32_t*>(p);
             else tail[j] = *reinterpret_cast<const uint16_t*>(p);
         }
@@ -180,6 +184,17 @@ template <> __device__ __forceinline__ float load_elem(const uint16_t* p) { retu
 template <> __device__ __forceinline__ float load_elem(const bf16_t* p) { return bf16_to_float(p->bits); }
 template <> __device__ __forceinline__ float load_elem(const float* p) { return *p; }
 
+// Four outputs, rounded once.
+__device__ __forceinline__ void store_out4(uint16_t* to, const f32x4_t& o) {
+    typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<f16x4_t*>(to) = __builtin_convertvector(o, f16x4_t);
+}
+__device__ __forceinline__ void store_out4(bf16_t* to, const f32x4_t& o) {
+    typedef uint16_t u16x4_t __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<u16x4_t*>(to) = u16x4_t{float_to_bf16(o[0]), float_to_bf16(o[1]), float_to_bf16(o[2]), float_to_bf16(o[3])};
+}
+__device__ __forceinline__ void store_out4(float* to, const f32x4_t& o) { *reinterpret_cast<f32x4_t*>(to) = o; }
+
 // Slots of sample b: [first, length).
 __device__ __forceinline__ void sample_range(const int* first_keys, const int* lengths, int b, int t, int* first, int* length) {
     const int n = lengths ? min(max(lengths[b], 0), t) : t;
@@ -206,14 +221,15 @@ __device__ __forceinline__ uint64_t ancestor_mask(const int* parents, int tokens
     return ((uint64_t)hi << 32) | lo;
 }
 
-struct Yes { static constexpr bool value = true; };
-struct No { static constexpr bool value = false; };
-
 // ---------------------------------------------------------------------------------------
+// Waves a SIMD that the registers are cut for.  Two hide a wave's loads and transcendentals behind the
+// other's matrix products; what holds more than 256 registers of results and operands runs alone.
+constexpr int tree_waves_per_simd(int dh, int rt) { return dh <= 128 && dh * rt <= 256 ? 2 : 1; }
+
 template <typename T, int DH, int RT>
-__global__ void __launch_bounds__(kTreeWaves * 64) ffa_tree_kernel(const TreeParams P) {
+__global__ void __launch_bounds__(kTreeWaves * 64, tree_waves_per_simd(DH, RT)) ffa_tree_kernel(const TreeParams P) {
     using G = TreeGeo<T, DH>;
-    constexpr int W = kTreeWaves, NU = G::NU, TK = G::TK, KK = G::KK, NCH = G::NCH, DB = G::DB;
+    constexpr int W = kTreeWaves, NU = G::NU, TK = G::TK, KK = G::KK, NCH = G::NCH, DB = G::DB, NJ = 4 * NU;
     constexpr int RS = DH + 4;  // floats of a row in the merge buffer
     __shared__ float s_acc[W][16 * RS];
     __shared__ float s_ml[W][RT * 16][2];
@@ -243,10 +259,78 @@ __global__ void __launch_bounds__(kTreeWaves * 64) ffa_tree_kernel(const TreePar
     const long long kn_row = P.k_stride[2] * (long long)sizeof(T), vn_row = P.v_stride[2] * (long long)sizeof(T);
     const int row0 = rb * RT * 16;
 
+    // This wave's tiles: wave, wave + W, ... of the piece's cached keys, then its share of the tiles
+    // of new tokens, which are dealt from the last wave on (the piece's shorter ends).
+    const int lo = max(split * P.tiles_per_split, first / TK) + wave;
+    const int hi = min((split + 1) * P.tiles_per_split, (length + TK - 1) / TK);
+    const int n_cached = max(0, (hi - lo + W - 1) / W);
+    const int n_new = last ? max(0, ((count + TK - 1) / TK + wave) / W) : 0;
+    const int n_tiles = n_cached + n_new;
+
+    uint4 kf[NU][KK];
+    VTile<T, DH> vt;
+    // A chunk that does not exist (Dh = 80) must not hold an infinity against the zero of Q.
+    auto existing = [&](const uint4& x, int kk) {
+        if (NCH % 4 != 0 && kk == KK - 1 && kk * 4 + g >= NCH) return make_uint4(0, 0, 0, 0);
+        return x;
+    };
+    // Tile i of this wave: its first key, counted in the cache or among the new tokens.
+    auto key0_of = [&](int i) { return (i < n_cached ? lo + i * W : W - 1 - wave + (i - n_cached) * W) * TK; };
+    // A whole tile of cached keys: uniform addresses plus one fixed offset a lane.  Any other tile:
+    // rows past the end are read from the last one, and masked.
+    const unsigned k_lane = ((unsigned)g * (unsigned)P.Lmax + (unsigned)c) * 16u;
+    const unsigned k_lane_end = ((unsigned)min(g, NCH - 1 - (KK - 1) * 4) * (unsigned)P.Lmax + (unsigned)c) * 16u;
+    const unsigned v_lane = (unsigned)g * 4u * (unsigned)cache_row;
+    auto whole_tile = [&](int i) { return i < n_cached && key0_of(i) + TK <= length; };
+    auto load_k = [&](int i) {
+        const int key0 = key0_of(i);
+        if (whole_tile(i)) {
+            const char* base = kc + (size_t)key0 * 16;
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                for (int u = 0; u < NU; ++u) {
+                    const char* from = base + (size_t)kk * 4 * P.Lmax * 16 + u * 256;
+                    kf[u][kk] = existing(ld16(from + (NCH % 4 != 0 && kk == KK - 1 ? k_lane_end : k_lane)), kk);
+                }
+        } else {
+            const bool cached = i < n_cached;
+            const char* base = cached ? kc : kn;
+            const long long row_step = cached ? 16 : kn_row, chunk_step = cached ? (long long)P.Lmax * 16 : 16;
+            const int end = (cached ? length : count) - 1;
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                const char* row = base + min(key0 + u * 16 + c, end) * row_step;
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) kf[u][kk] = existing(ld16(row + min(kk * 4 + g, NCH - 1) * chunk_step), kk);
+            }
+        }
+    };
+    auto load_v = [&](int i) {
+        const int key0 = key0_of(i);
+        if (whole_tile(i)) {
+            const char* base = vc + (size_t)key0 * cache_row;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) vt.load(j, base + ((j / 4) * 16 + j % 4) * cache_row, v_lane, c);
+        } else {
+            const bool cached = i < n_cached;
+            const char* base = cached ? vc : vn;
+            const long long step = cached ? (long long)cache_row : vn_row;
+            const int end = (cached ? length : count) - 1;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) vt.load(j, base + min(key0 + (j / 4) * 16 + g * 4 + j % 4, end) * step, 0u, c);
+        }
+    };
+    if (n_tiles > 0) {
+        load_k(0);
+        load_v(0);
+    }
+
     if (tid < 2) s_bad[tid] = 0;
-    if (wave == 0) s_seen[lane] = ancestor_mask(P.parents ? P.parents + (size_t)b * P.tokens : nullptr, P.tokens, lane);
+    if (last && wave == 0) s_seen[lane] = ancestor_mask(P.parents ? P.parents + (size_t)b * P.tokens : nullptr, P.tokens, lane);
 
     // Q: chunk kk * 4 + g of row row0 + rt * 16 + c; rows and chunks that do not exist are zero.
+    // The factor of the scores is positive: a negative softmax_scale turns Q's sign.
     uint4 qf[RT][KK];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -258,7 +342,13 @@ __global__ void __launch_bounds__(kTreeWaves * 64) ffa_tree_kernel(const TreePar
         for (int kk = 0; kk < KK; ++kk) {
             const int ch = kk * 4 + g;
             qf[rt][kk] = make_uint4(0, 0, 0, 0);
-            if (row < P.rows && ch < NCH) qf[rt][kk] = *reinterpret_cast<const uint4*>(qr + ch * 16);
+            if (row < P.rows && ch < NCH && P.q_sign != 0) {
+                constexpr uint32_t sign = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+                const uint32_t turn = P.q_sign < 0 ? sign : 0u;
+                uint4 x = *reinterpret_cast<const uint4*>(qr + ch * 16);
+                x.x ^= turn; x.y ^= turn; x.z ^= turn; x.w ^= turn;
+                qf[rt][kk] = x;
+            }
         }
     }
     __syncthreads();
@@ -273,42 +363,10 @@ __global__ void __launch_bounds__(kTreeWaves * 64) ffa_tree_kernel(const TreePar
         for (int db = 0; db < DB; ++db) acc[rt][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 
-    uint4 kf[NU][KK];
-    VTile<T, DH> vt;
-
-    // A chunk that does not exist (Dh = 80) must not hold an infinity against the zero of Q.
-    auto existing = [&](const uint4& x, int kk) {
-        if (NCH % 4 != 0 && kk == KK - 1 && kk * 4 + g >= NCH) return make_uint4(0, 0, 0, 0);
-        return x;
-    };
-    // The loads of a tile of cached keys.  Slots past the sample's end are read from its last slot.
-    auto load_k = [&](int tile) {
-        const int key0 = tile * TK;
-#pragma unroll
-        for (int u = 0; u < NU; ++u) {
-            const int key = min(key0 + u * 16 + c, length - 1);
-#pragma unroll
-            for (int kk = 0; kk < KK; ++kk) {
-                const int gg = NCH % 4 != 0 && kk == KK - 1 ? min(g, NCH - 1 - kk * 4) : g;
-                const char* base = kc + (size_t)kk * 4 * P.Lmax * 16;
-                kf[u][kk] = existing(ld16(base + ((unsigned)gg * (unsigned)P.Lmax + (unsigned)key) * 16u), kk);
-            }
-        }
-    };
-    auto load_v = [&](int tile) {
-        const int key0 = tile * TK;
-        const char* base = vc + (size_t)key0 * cache_row;
-        const int most = length - 1 - key0;
-#pragma unroll
-        for (int j = 0; j < 4 * NU; ++j) {
-            const int k = (j / 4) * 16 + g * 4 + j % 4;
-            vt.load(j, base + (unsigned)min(k, most) * (unsigned)cache_row, c);
-        }
-    };
-
-    // One tile: scores, weights, products.  seen(row tile, key of the tile) is asked if `masked`.
-    auto tile_step = [&](auto masked, auto seen, int score_key, auto next_k, auto next_v) {
-        constexpr bool MASKED = decltype(masked)::value;
+    for (int i = 0; i < n_tiles; ++i) {
+        const int key0 = key0_of(i);
+        const bool cached = i < n_cached;
+        const bool masked = !cached || key0 < first || key0 + TK > length;
         f32x4_t s[RT][NU];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -318,26 +376,63 @@ __global__ void __launch_bounds__(kTreeWaves * 64) ffa_tree_kernel(const TreePar
 #pragma unroll
                 for (int kk = 0; kk < KK; ++kk) s[rt][u] = mma_qk(kf[u][kk], qf[rt][kk], s[rt][u], T{});
             }
-        next_k();
+        if (i + 1 < n_tiles) load_k(i + 1);
+        if (masked) {
+            // Bit j: this lane's key j is seen.  Cached keys: the sample's range; new ones: ancestors.
+            auto bits_of = [&](uint64_t range) {
+                uint32_t x = (uint32_t)(range >> (g * 4)) & 15u;
+                if (NU == 2) x |= ((uint32_t)(range >> (16 + g * 4)) & 15u) << 4;
+                return x;
+            };
+            uint64_t range = 0;
+            if (cached) {
+                const int from = max(first - key0, 0), to = min(length - key0, TK);
+                range = ((1ull << to) - 1) & ~((1ull << from) - 1);
+            }
+            uint32_t held = cached ? bits_of(range) : 0;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const int row = row0 + rt * 16 + c;
+                const uint32_t bits = cached ? held : row < P.rows ? bits_of(s_seen[row / P.G] >> key0) : 0u;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+                    if (!(bits >> j & 1)) s[rt][j / 4][j % 4] = -INFINITY;
+            }
+            // V of what no row sees must not meet a zero weight: 0 * NaN.  An infinite or NaN value of a
+            // new token is added at the end, to the rows that see it.
+            if (cached) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+                    if (!(held >> j & 1)) vt.clear(j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    const int node = key0 + (j / 4) * 16 + g * 4 + j % 4;
+                    if (node >= count) vt.clear(j);
+                    else if (vt.drop_nonfinite(j)) atomicOr(&s_bad[node / 32], 1u << (node % 32));
+                }
+            }
+        }
+        if (P.ws_scores != nullptr) {
+            const int at = cached ? key0 : P.score_stride - 32;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const int row = row0 + rt * 16 + c;
+                if (row < P.rows) {
+                    float* to = P.ws_scores + ((size_t)pair * P.rows + row) * P.score_stride + at + g * 4;
+#pragma unroll
+                    for (int u = 0; u < NU; ++u) *reinterpret_cast<f32x4_t*>(to + u * 16) = s[rt][u] * P.scale_log2e;
+                }
+            }
+        }
         PFrag16 pf[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            float x[4 * NU], top = -INFINITY;
+            float x[NJ];
+            float top = s[rt][0][0];
 #pragma unroll
-            for (int j = 0; j < 4 * NU; ++j) {
-                x[j] = s[rt][j / 4][j % 4] * P.scale_log2e;
-                if (MASKED && !seen(rt, (j / 4) * 16 + g * 4 + j % 4)) x[j] = -INFINITY;
-                top = fmaxf(top, x[j]);
-            }
-            if (P.ws_scores != nullptr) {
-                const int row = row0 + rt * 16 + c;
-                if (row < P.rows) {
-                    float* to = P.ws_scores + ((size_t)pair * P.rows + row) * P.score_stride + score_key + g * 4;
-#pragma unroll
-                    for (int u = 0; u < NU; ++u)
-                        *reinterpret_cast<float4*>(to + u * 16) = make_float4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
-                }
-            }
+            for (int j = 1; j < NJ; ++j) top = fmaxf(top, s[rt][j / 4][j % 4]);
+            top *= P.scale_log2e;
             if (__any(top > m[rt] + kSlack)) {
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
@@ -348,11 +443,11 @@ __global__ void __launch_bounds__(kTreeWaves * 64) ffa_tree_kernel(const TreePar
 #pragma unroll
                 for (int db = 0; db < DB; ++db) acc[rt][db] *= f;
             }
-            const float ref = m[rt] == -INFINITY ? 0.f : m[rt];
+            const float ref = m[rt] == -INFINITY ? 0.f : -m[rt];
             float sum = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4 * NU; ++j) {
-                x[j] = __builtin_amdgcn_exp2f(x[j] - ref);
+            for (int j = 0; j < NJ; ++j) {
+                x[j] = __builtin_amdgcn_exp2f(fmaf(s[rt][j / 4][j % 4], P.scale_log2e, ref));
                 sum += x[j];
             }
             l[rt] += sum;
@@ -381,63 +476,7 @@ __global__ void __launch_bounds__(kTreeWaves * 64) ffa_tree_kernel(const TreePar
                         acc[rt][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(vt.at(j, blk, e), s[rt][0][j], acc[rt][db], 0, 0, 0);
             }
         }
-        next_v();
-    };
-    // ---- cached keys: tiles wave, wave + W, ... of the piece ----
-    {
-        const int lo = max(split * P.tiles_per_split, first / TK);
-        const int hi = min((split + 1) * P.tiles_per_split, (length + TK - 1) / TK);
-        int tile = lo + wave;
-        if (tile < hi) {
-            load_k(tile);
-            load_v(tile);
-        }
-        for (; tile < hi; tile += W) {
-            const int key0 = tile * TK, next = tile + W;
-            auto nk = [&]() { if (next < hi) load_k(next); };
-            auto nv = [&]() { if (next < hi) load_v(next); };
-            if (key0 >= first && key0 + TK <= length) {
-                tile_step(No{}, [](int, int) { return true; }, key0, nk, nv);
-            } else {
-                auto real = [&](int k) { return key0 + k >= first && key0 + k < length; };
-#pragma unroll
-                for (int j = 0; j < 4 * NU; ++j)
-                    if (!real((j / 4) * 16 + g * 4 + j % 4)) vt.clear(j);
-                tile_step(Yes{}, [&](int, int k) { return real(k); }, key0, nk, nv);
-            }
-        }
-    }
-
-    // ---- the new tokens themselves, dealt to the waves from the last: the piece's shorter ends ----
-    if (last) {
-        const int tiles = (count + TK - 1) / TK;
-        for (int d = W - 1 - wave; d < tiles; d += W) {
-            const int node0 = d * TK;
-#pragma unroll
-            for (int u = 0; u < NU; ++u) {
-                const int node = min(node0 + u * 16 + c, count - 1);
-#pragma unroll
-                for (int kk = 0; kk < KK; ++kk) {
-                    const int ch = min(kk * 4 + g, NCH - 1);
-                    kf[u][kk] = existing(*reinterpret_cast<const uint4*>(kn + node * kn_row + ch * 16), kk);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 4 * NU; ++j) {
-                const int node = node0 + (j / 4) * 16 + g * 4 + j % 4;
-                vt.load(j, vn + min(node, count - 1) * vn_row, c);
-                // What is not finite is added at the end, to the rows that see it.
-                if (node >= count) vt.clear(j);
-                else if (vt.drop_nonfinite(j)) atomicOr(&s_bad[node / 32], 1u << (node % 32));
-            }
-            uint64_t mask[RT];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const int row = row0 + rt * 16 + c;
-                mask[rt] = row < P.rows ? s_seen[row / P.G] >> node0 : 0;
-            }
-            tile_step(Yes{}, [&](int rt, int k) { return (bool)((mask[rt] >> k) & 1); }, P.score_stride - 32, [] {}, [] {});
-        }
+        if (i + 1 < n_tiles) load_v(i + 1);
     }
 
     // ---- join the waves ----
@@ -506,8 +545,7 @@ __global__ void __launch_bounds__(kTreeWaves * 64) ffa_tree_kernel(const TreePar
             } else if (token < count) {
                 const int gh = row % P.G;
                 T* to = static_cast<T*>(P.out) + b * P.out_stride[0] + (long long)(h * P.G + gh) * P.out_stride[1] + token * P.out_stride[2];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) store_out(to, d + e, o[e] / L);
+                store_out4(to + d, o / L);
             }
         }
     }
@@ -550,8 +588,7 @@ __global__ void __launch_bounds__(256) ffa_tree_join_kernel(const TreeParams P) 
         o += *reinterpret_cast<const f32x4_t*>(P.ws_acc + slot * DH + d) * f;
     }
     T* to = static_cast<T*>(P.out) + b * P.out_stride[0] + (long long)(h * P.G + row % P.G) * P.out_stride[1] + token * P.out_stride[2];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) store_out(to, d + e, o[e] / L);
+    store_out4(to + d, o / L);
 }
 
 // Weight-summing step, after the scores and the pieces' (m, l) are known: every key's weight.
