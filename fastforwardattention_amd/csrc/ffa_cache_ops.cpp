@@ -46,24 +46,36 @@ TreeSizes tree_sizes(int pairs, int rows, int head_dim, int n_splits, bool score
     return s;
 }
 
-int most_splits(int precision, int pairs, int row_blocks, int t, int cus) {
-    const int tiles = ceil_div(t, tree_tile_keys(precision));
-    // About four workgroups a CU hide the memory's latency; a piece has two tiles a wave at least,
-    // or its prologue and the merge cost more than the tiles.
-    const int want = ceil_div(4 * cus, pairs * row_blocks);
-    return std::max(1, std::min({want, tiles / (2 * kTreeWaves), 128}));
-}
+// Scores of a piece are held in LDS, next to the merge buffer, up to this many words.
+constexpr int kScoreLdsWords = 16384;
 
-int row_blocks_of(int rows, int head_dim) {
-    // Row tiles a wave can hold: Dh = 256 fills the registers with two.
-    return ceil_div(ceil_div(rows, 16), head_dim == 256 ? 2 : 4);
+struct TreeShape {
+    int row_tiles, row_blocks, waves, most_splits;
+};
+
+// What does not depend on the cut of the keys.  most_splits grows with t.
+TreeShape tree_shape(int precision, int pairs, int rows, int head_dim, int t, int cus) {
+    TreeShape s;
+    const int row_tiles = ceil_div(rows, 16);
+    s.row_blocks = ceil_div(row_tiles, tree_row_tiles(head_dim));
+    s.row_tiles = ceil_div(row_tiles, s.row_blocks);
+    const int tiles = ceil_div(t, tree_tile_keys(precision));
+    const int wide = tree_wide_waves(head_dim, s.row_tiles);
+    // One workgroup a CU streams at the memory's rate (measured from 1/4 to 16 a CU: 8 heads x 20000 keys
+    // 167, 95, 63, 84, 117 us at 1/4, 1/2, 1, 2, 4), more only add partial results to join.  Where pairs and
+    // row blocks are fewer than the CUs, workgroups have as many waves as a CU holds.
+    const int groups = pairs * s.row_blocks;
+    s.waves = wide != 0 && groups < cus ? wide : 4;
+    s.most_splits = std::max(1, std::min({ceil_div(cus, groups), tiles / (2 * s.waves), 128}));
+    return s;
 }
 
 int run_tree(int precision, int head_dim, TreeParams& P, void* workspace, size_t workspace_bytes, void* stream) {
     const int pairs = P.B * P.H;
-    const TreePlan plan = plan_tree(precision, pairs, P.rows, head_dim, P.t, compute_units());
     const bool scores = P.key_weights != nullptr;
-    const int most = most_splits(precision, pairs, plan.row_blocks, P.t, compute_units());
+    const int cus = compute_units();
+    const TreePlan plan = plan_tree(precision, pairs, P.rows, head_dim, P.t, scores, cus);
+    const int most = tree_shape(precision, pairs, P.rows, head_dim, P.t, cus).most_splits;
     const TreeSizes s = tree_sizes(pairs, P.rows, head_dim, most, scores, P.t);
     if (s.total() > 0) {
         if (workspace == nullptr || workspace_bytes < s.total()) return FFA_ERR_WORKSPACE;
@@ -74,6 +86,7 @@ int run_tree(int precision, int head_dim, TreeParams& P, void* workspace, size_t
     P.ws_ml = reinterpret_cast<float*>(base + s.acc);
     P.ws_scores = scores ? reinterpret_cast<float*>(base + s.acc + s.ml) : nullptr;
     P.score_stride = score_stride_of(P.t);
+    P.score_lds = plan.score_lds;
     P.n_splits = plan.n_splits;
     P.tiles_per_split = plan.tiles_per_split;
     P.row_blocks = plan.row_blocks;
@@ -98,7 +111,7 @@ size_t tree_workspace(int precision, int B, int H, int Hq, int Dh, int tokens, i
         return 0;
     const long long rows = (long long)(Hq / H) * tokens;
     if (rows > (1 << 20)) return 0;
-    const int n = most_splits(precision, B * H, row_blocks_of((int)rows, Dh), t, compute_units());
+    const int n = tree_shape(precision, B * H, (int)rows, Dh, t, compute_units()).most_splits;
     return tree_sizes(B * H, (int)rows, Dh, n, scores, t).total();
 }
 
@@ -111,14 +124,17 @@ bool overlap(const void* a, size_t na, const void* b, size_t nb) {
 
 namespace ffa {
 
-TreePlan plan_tree(int precision, int pairs, int rows, int head_dim, int t, int cus) {
+TreePlan plan_tree(int precision, int pairs, int rows, int head_dim, int t, bool weights, int cus) {
+    const TreeShape shape = tree_shape(precision, pairs, rows, head_dim, t, cus);
     TreePlan p;
-    p.row_blocks = row_blocks_of(rows, head_dim);
-    p.row_tiles = ceil_div(ceil_div(rows, 16), p.row_blocks);
-    const int tiles = ceil_div(t, tree_tile_keys(precision));
-    const int n = most_splits(precision, pairs, p.row_blocks, t, cus);
-    p.tiles_per_split = std::max(1, ceil_div(tiles, n));
+    p.row_tiles = shape.row_tiles;
+    p.row_blocks = shape.row_blocks;
+    p.waves = shape.waves;
+    const int tile = tree_tile_keys(precision), tiles = ceil_div(t, tile);
+    p.tiles_per_split = std::max(1, ceil_div(tiles, shape.most_splits));
     p.n_splits = std::max(1, ceil_div(tiles, p.tiles_per_split));
+    const long long words = (long long)p.tiles_per_split * tile + 32;
+    p.score_lds = weights && rows <= 16 && words * rows <= kScoreLdsWords ? (int)words : 0;
     return p;
 }
 

@@ -11,18 +11,28 @@ namespace ffa {
 
 // ---------------------------------------------------------------------------------------
 // Attention of a group of tokens.  The rows of a (sample, cache head) pair -- its tokens times
-// its G query heads, row = token * G + head -- are cut into blocks of row_tiles * 16; a
-// workgroup of kTreeWaves waves takes one row block over one piece of the keys.
-constexpr int kTreeWaves = 4;
+// its G query heads, row = token * G + head -- are cut into blocks of row_tiles * 16; a workgroup
+// takes one row block over one piece of the keys, its waves every n-th tile of them.
 
 // Keys of one wave tile: two (16-bit) or one (fp32) matrix tiles of 16 keys.
 inline int tree_tile_keys(int precision) { return precision == FFA_PRECISION_F32 ? 16 : 32; }
 
+// Most 16-row matrix tiles a wave holds without spilling registers.
+constexpr int tree_row_tiles(int head_dim) { return head_dim == 256 ? 2 : head_dim == 128 ? 3 : 4; }
+
+// Waves of a workgroup where the pairs alone do not fill the chip: what the registers of the kernel
+// let a CU hold (0: no such kernel).  Elsewhere workgroups have 4.
+constexpr int tree_wide_waves(int head_dim, int row_tiles) {
+    return head_dim == 64 && row_tiles == 1 ? 16 : head_dim * row_tiles <= 128 ? 8 : 0;
+}
+
 struct TreePlan {
     int row_tiles;        // 16-row matrix tiles a wave holds: 1 .. 4
     int row_blocks;       // workgroups a piece of keys is read by
+    int waves;            // of a workgroup: 4, or tree_wide_waves()
     int n_splits;         // pieces of the cached keys
     int tiles_per_split;  // wave tiles a piece holds
+    int score_lds;        // weight-summing step: words of a row of scores held in LDS, 0 = in the workspace
 };
 
 struct TreeParams {
@@ -35,17 +45,18 @@ struct TreeParams {
     float* ws_scores;    // weight-summing step: [pairs, rows, score_stride], else nullptr
     float* key_weights;  // weight-summing step: [pairs, Lmax], else nullptr
     int score_stride;
+    int score_lds;       // as in the plan
     int B, H, G, tokens, rows, Lmax, t;
     float scale_log2e;  // |softmax_scale| * log2(e), never zero
     int q_sign;         // sign of softmax_scale: Q enters with it
     int n_splits, tiles_per_split, row_blocks;
 };
 
-TreePlan plan_tree(int precision, int pairs, int rows, int head_dim, int t, int cus);
+TreePlan plan_tree(int precision, int pairs, int rows, int head_dim, int t, bool weights, int cus);
 int launch_tree(int precision, int head_dim, const TreeParams& P, const TreePlan& plan, void* stream);
-int launch_tree_f16(const TreeParams& P, int head_dim, int row_tiles, void* stream);
-int launch_tree_bf16(const TreeParams& P, int head_dim, int row_tiles, void* stream);
-int launch_tree_f32(const TreeParams& P, int head_dim, int row_tiles, void* stream);
+int launch_tree_f16(const TreeParams& P, int head_dim, const TreePlan& plan, void* stream);
+int launch_tree_bf16(const TreeParams& P, int head_dim, const TreePlan& plan, void* stream);
+int launch_tree_f32(const TreeParams& P, int head_dim, const TreePlan& plan, void* stream);
 
 // ---------------------------------------------------------------------------------------
 // Moves of cache slots.  Pointers of up to kSlotCaches caches travel in the kernel arguments.

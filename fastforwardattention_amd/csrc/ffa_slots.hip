@@ -10,9 +10,9 @@
 namespace ffa {
 
 int launch_tree(int precision, int head_dim, const TreeParams& P, const TreePlan& plan, void* stream) {
-    if (precision == FFA_PRECISION_F16) return launch_tree_f16(P, head_dim, plan.row_tiles, stream);
-    if (precision == FFA_PRECISION_BF16) return launch_tree_bf16(P, head_dim, plan.row_tiles, stream);
-    return launch_tree_f32(P, head_dim, plan.row_tiles, stream);
+    if (precision == FFA_PRECISION_F16) return launch_tree_f16(P, head_dim, plan, stream);
+    if (precision == FFA_PRECISION_BF16) return launch_tree_bf16(P, head_dim, plan, stream);
+    return launch_tree_f32(P, head_dim, plan, stream);
 }
 
 // ---------------------------------------------------------------------------------------

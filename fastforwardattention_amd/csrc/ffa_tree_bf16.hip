@@ -3,8 +3,8 @@
 
 namespace ffa {
 
-int launch_tree_bf16(const TreeParams& P, int head_dim, int row_tiles, void* stream) {
-    return launch_tree_type<bf16_t>(P, head_dim, row_tiles, stream);
+int launch_tree_bf16(const TreeParams& P, int head_dim, const TreePlan& plan, void* stream) {
+    return launch_tree_type<bf16_t>(P, head_dim, plan, stream);
 }
 
 }  // namespace ffa

@@ -3,8 +3,8 @@
 
 namespace ffa {
 
-int launch_tree_f32(const TreeParams& P, int head_dim, int row_tiles, void* stream) {
-    return launch_tree_type<float>(P, head_dim, row_tiles, stream);
+int launch_tree_f32(const TreeParams& P, int head_dim, const TreePlan& plan, void* stream) {
+    return launch_tree_type<float>(P, head_dim, plan, stream);
 }
 
 }  // namespace ffa

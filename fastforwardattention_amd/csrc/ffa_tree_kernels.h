@@ -224,15 +224,21 @@ __device__ __forceinline__ uint64_t ancestor_mask(const int* parents, int tokens
 // ---------------------------------------------------------------------------------------
 // Waves a SIMD that the registers are cut for.  Two hide a wave's loads and transcendentals behind the
 // other's matrix products; what holds more than 256 registers of results and operands runs alone.
-constexpr int tree_waves_per_simd(int dh, int rt) { return dh <= 128 && dh * rt <= 256 ? 2 : 1; }
+constexpr int tree_waves_per_simd(int dh, int rt, int w) { return w > 4 ? w / 4 : dh <= 128 && dh * rt <= 256 ? 2 : 1; }
 
-template <typename T, int DH, int RT>
-__global__ void __launch_bounds__(kTreeWaves * 64, tree_waves_per_simd(DH, RT)) ffa_tree_kernel(const TreeParams P) {
+// Floats of LDS in front of the scores: the waves' results of one row tile.
+template <int DH, int W> constexpr int tree_merge_floats() { return W * 16 * (DH + 4); }
+
+template <typename T, int DH, int RT, int W>
+__global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT, W)) ffa_tree_kernel(const TreeParams P) {
     using G = TreeGeo<T, DH>;
-    constexpr int W = kTreeWaves, NU = G::NU, TK = G::TK, KK = G::KK, NCH = G::NCH, DB = G::DB, NJ = 4 * NU;
+    constexpr int NU = G::NU, TK = G::TK, KK = G::KK, NCH = G::NCH, DB = G::DB, NJ = 4 * NU;
     constexpr int RS = DH + 4;  // floats of a row in the merge buffer
-    __shared__ float s_acc[W][16 * RS];
+    extern __shared__ float4 s_dynamic[];
+    float* const s_acc = reinterpret_cast<float*>(s_dynamic);     // [W][16 * RS]
+    float* const s_scores = s_acc + tree_merge_floats<DH, W>();   // [rows][score_lds], weight-summing step
     __shared__ float s_ml[W][RT * 16][2];
+    __shared__ float s_row[16][2];  // weight-summing step: -M and 1 / L of a row
     __shared__ uint64_t s_seen[64];
     __shared__ unsigned s_bad[2];
 
@@ -261,6 +267,7 @@ __global__ void __launch_bounds__(kTreeWaves * 64, tree_waves_per_simd(DH, RT)) 
 
     // This wave's tiles: wave, wave + W, ... of the piece's cached keys, then its share of the tiles
     // of new tokens, which are dealt from the last wave on (the piece's shorter ends).
+    const int piece0 = split * P.tiles_per_split * TK;
     const int lo = max(split * P.tiles_per_split, first / TK) + wave;
     const int hi = min((split + 1) * P.tiles_per_split, (length + TK - 1) / TK);
     const int n_cached = max(0, (hi - lo + W - 1) / W);
@@ -414,14 +421,17 @@ __global__ void __launch_bounds__(kTreeWaves * 64, tree_waves_per_simd(DH, RT)) 
             }
         }
         if (P.ws_scores != nullptr) {
-            const int at = cached ? key0 : P.score_stride - 32;
+            // In LDS if the piece's fit (key - first key of the piece), else in the workspace; the new
+            // token's scores lie in the last 32 words.
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 const int row = row0 + rt * 16 + c;
                 if (row < P.rows) {
-                    float* to = P.ws_scores + ((size_t)pair * P.rows + row) * P.score_stride + at + g * 4;
+                    float* to = P.score_lds != 0
+                                    ? s_scores + row * P.score_lds + (cached ? key0 - piece0 : P.score_lds - 32)
+                                    : P.ws_scores + ((size_t)pair * P.rows + row) * P.score_stride + (cached ? key0 : P.score_stride - 32);
 #pragma unroll
-                    for (int u = 0; u < NU; ++u) *reinterpret_cast<f32x4_t*>(to + u * 16) = s[rt][u] * P.scale_log2e;
+                    for (int u = 0; u < NU; ++u) *reinterpret_cast<f32x4_t*>(to + g * 4 + u * 16) = s[rt][u] * P.scale_log2e;
                 }
             }
         }
@@ -505,7 +515,7 @@ __global__ void __launch_bounds__(kTreeWaves * 64, tree_waves_per_simd(DH, RT)) 
         for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                s_acc[wave][c * RS + tile_dim<T, DH>(db, g * 4 + r)] = m[rt] == -INFINITY ? 0.f : acc[rt][db][r] * f;
+                s_acc[wave * 16 * RS + c * RS + tile_dim<T, DH>(db, g * 4 + r)] = m[rt] == -INFINITY ? 0.f : acc[rt][db][r] * f;
         __syncthreads();
         // 16 rows x DH outputs, four dims a thread.
         for (int i = tid; i < 16 * DH / 4; i += W * 64) {
@@ -522,7 +532,7 @@ __global__ void __launch_bounds__(kTreeWaves * 64, tree_waves_per_simd(DH, RT)) 
             for (int w = 0; w < W; ++w) {
                 const float mw = s_ml[w][rt * 16 + r][0];
                 if (mw != -INFINITY) L += s_ml[w][rt * 16 + r][1] * __builtin_amdgcn_exp2f(mw - M);
-                o += *reinterpret_cast<const f32x4_t*>(&s_acc[w][r * RS + d]);
+                o += *reinterpret_cast<const f32x4_t*>(&s_acc[w * 16 * RS + r * RS + d]);
             }
             if (bad != 0) {
                 for (uint64_t todo = bad & s_seen[token]; todo != 0; todo &= todo - 1) {
@@ -536,6 +546,10 @@ __global__ void __launch_bounds__(kTreeWaves * 64, tree_waves_per_simd(DH, RT)) 
                 }
             }
             const size_t slot = ((size_t)pair * P.n_splits + split) * P.rows + row;
+            if (P.ws_scores != nullptr && P.score_lds != 0 && d == 0) {
+                s_row[r][0] = -M;
+                s_row[r][1] = 1.f / L;
+            }
             if ((!whole || P.ws_scores != nullptr) && d == 0) {
                 P.ws_ml[slot * 2] = M;
                 P.ws_ml[slot * 2 + 1] = L;
@@ -546,6 +560,29 @@ __global__ void __launch_bounds__(kTreeWaves * 64, tree_waves_per_simd(DH, RT)) 
                 const int gh = row % P.G;
                 T* to = static_cast<T*>(P.out) + b * P.out_stride[0] + (long long)(h * P.G + gh) * P.out_stride[1] + token * P.out_stride[2];
                 store_out4(to + d, o / L);
+            }
+        }
+    }
+
+    // ---- weight-summing step with scores in LDS (one row tile): the weights if this piece is all there
+    // is, else the scores go to the workspace, where the pieces' kernel finds them ----
+    if (P.ws_scores != nullptr && P.score_lds != 0) {
+        __syncthreads();
+        const int from = max(first, piece0), to = min(length, piece0 + P.tiles_per_split * TK);
+        if (whole) {
+            float* kw = P.key_weights + (size_t)pair * P.Lmax;
+            for (int j = from + tid; j <= to; j += W * 64) {
+                float w = 0.f;
+                for (int r = 0; r < P.rows; ++r)
+                    w += __builtin_amdgcn_exp2f(s_scores[r * P.score_lds + (j == length ? P.score_lds - 32 : j - piece0)] + s_row[r][0]) * s_row[r][1];
+                if (j == length) kw[j] = w;
+                else kw[j] += w;
+            }
+        } else {
+            for (int r = 0; r < P.rows; ++r) {
+                float* ws = P.ws_scores + ((size_t)pair * P.rows + r) * P.score_stride;
+                for (int j = from + tid; j < to; j += W * 64) ws[j] = s_scores[r * P.score_lds + j - piece0];
+                if (last && tid == 0) ws[P.score_stride - 32] = s_scores[r * P.score_lds + P.score_lds - 32];
             }
         }
     }
@@ -564,93 +601,129 @@ __global__ void __launch_bounds__(kTreeWaves * 64, tree_waves_per_simd(DH, RT)) 
     }
 }
 
-// Joins the pieces of a row: out = sum_i O_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).  Four dims a thread.
-template <typename T, int DH>
-__global__ void __launch_bounds__(256) ffa_tree_join_kernel(const TreeParams P) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long line = i / (DH / 4);
-    const int d = (int)(i % (DH / 4)) * 4;
-    if (line >= (long long)P.B * P.H * P.rows) return;
-    const int pair = (int)(line / P.rows), row = (int)(line % P.rows);
-    const int b = pair / P.H, h = pair % P.H, token = row / P.G;
-    if (P.counts && token >= P.counts[b]) return;
-    const size_t slot0 = (size_t)pair * P.n_splits * P.rows + row;
-    float M = -INFINITY;
-    for (int s = 0; s < P.n_splits; ++s) M = fmaxf(M, P.ws_ml[(slot0 + (size_t)s * P.rows) * 2]);
-    float L = 0.f;
-    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+// After the pieces.  The first join_blocks workgroups join the rows, four dims a thread:
+// out = sum_i O_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).  The others turn scores into weights: 256 keys of
+// a pair each.
+struct RowTotal { float M, L; };
+__device__ __forceinline__ RowTotal row_total(const TreeParams& P, size_t slot0) {
+    RowTotal t = {-INFINITY, 0.f};
+    for (int s = 0; s < P.n_splits; ++s) t.M = fmaxf(t.M, P.ws_ml[(slot0 + (size_t)s * P.rows) * 2]);
     for (int s = 0; s < P.n_splits; ++s) {
-        const size_t slot = slot0 + (size_t)s * P.rows;
-        const float ms = P.ws_ml[slot * 2];
-        if (ms == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(ms - M);
-        L += P.ws_ml[slot * 2 + 1] * f;
-        o += *reinterpret_cast<const f32x4_t*>(P.ws_acc + slot * DH + d) * f;
+        const float ms = P.ws_ml[(slot0 + (size_t)s * P.rows) * 2];
+        if (ms != -INFINITY) t.L += P.ws_ml[(slot0 + (size_t)s * P.rows) * 2 + 1] * __builtin_amdgcn_exp2f(ms - t.M);
     }
-    T* to = static_cast<T*>(P.out) + b * P.out_stride[0] + (long long)(h * P.G + row % P.G) * P.out_stride[1] + token * P.out_stride[2];
-    store_out4(to + d, o / L);
+    return t;
 }
 
-// Weight-summing step, after the scores and the pieces' (m, l) are known: every key's weight.
-static __global__ void __launch_bounds__(256) ffa_tree_weights_kernel(const TreeParams P, int blocks) {
-    const int pair = blockIdx.x / blocks, b = pair / P.H;
+template <typename T, int DH>
+__global__ void __launch_bounds__(256) ffa_tree_finish_kernel(const TreeParams P, int join_blocks, int key_blocks) {
+    if ((int)blockIdx.x < join_blocks) {
+        const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+        const long long line = i / (DH / 4);
+        const int d = (int)(i % (DH / 4)) * 4;
+        if (line >= (long long)P.B * P.H * P.rows) return;
+        const int pair = (int)(line / P.rows), row = (int)(line % P.rows);
+        const int b = pair / P.H, h = pair % P.H, token = row / P.G;
+        if (P.counts && token >= P.counts[b]) return;
+        const size_t slot0 = (size_t)pair * P.n_splits * P.rows + row;
+        // Eight pieces' loads at a time: a few rows are all there is to hide their latency.
+        constexpr int U = 8;
+        float M = -INFINITY, L = 0.f;
+        f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+        for (int s0 = 0; s0 < P.n_splits; s0 += U) {
+            float ms[U], ls[U];
+            f32x4_t os[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const size_t slot = slot0 + (size_t)min(s0 + u, P.n_splits - 1) * P.rows;
+                ms[u] = P.ws_ml[slot * 2];
+                ls[u] = P.ws_ml[slot * 2 + 1];
+                os[u] = *reinterpret_cast<const f32x4_t*>(P.ws_acc + slot * DH + d);
+            }
+            float top = M;
+#pragma unroll
+            for (int u = 0; u < U; ++u) top = s0 + u < P.n_splits ? fmaxf(top, ms[u]) : top;
+            if (M != -INFINITY) {
+                const float f = __builtin_amdgcn_exp2f(M - top);
+                L *= f;
+                o *= f;
+            }
+            M = top;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (s0 + u >= P.n_splits || ms[u] == -INFINITY) continue;
+                const float f = __builtin_amdgcn_exp2f(ms[u] - M);
+                L += ls[u] * f;
+                o += os[u] * f;
+            }
+        }
+        T* to = static_cast<T*>(P.out) + b * P.out_stride[0] + (long long)(h * P.G + row % P.G) * P.out_stride[1] + token * P.out_stride[2];
+        store_out4(to + d, o / L);
+        return;
+    }
+    const int block = blockIdx.x - join_blocks;
+    const int pair = block / key_blocks, b = pair / P.H;
     int first, length;
     sample_range(P.first_keys, P.lengths, b, P.t, &first, &length);
-    const int j = (blockIdx.x % blocks) * 256 + threadIdx.x;
-    if (j > length) return;
+    const int j = (block % key_blocks) * 256 + threadIdx.x;
+    if (j > length || j < first) return;
     float w = 0.f;
     for (int row = 0; row < P.rows; ++row) {
-        const size_t slot0 = (size_t)pair * P.n_splits * P.rows + row;
-        float M = -INFINITY, L = 0.f;
-        for (int s = 0; s < P.n_splits; ++s) M = fmaxf(M, P.ws_ml[(slot0 + (size_t)s * P.rows) * 2]);
-        for (int s = 0; s < P.n_splits; ++s) {
-            const float ms = P.ws_ml[(slot0 + (size_t)s * P.rows) * 2];
-            if (ms != -INFINITY) L += P.ws_ml[(slot0 + (size_t)s * P.rows) * 2 + 1] * __builtin_amdgcn_exp2f(ms - M);
-        }
+        const RowTotal t = row_total(P, (size_t)pair * P.n_splits * P.rows + row);
         const float* x = P.ws_scores + ((size_t)pair * P.rows + row) * P.score_stride;
-        if (j >= first) w += __builtin_amdgcn_exp2f(x[j == length ? P.score_stride - 32 : j] - M) / L;
+        w += __builtin_amdgcn_exp2f(x[j == length ? P.score_stride - 32 : j] - t.M) / t.L;
     }
     float* to = P.key_weights + (size_t)pair * P.Lmax + j;
     if (j == length) *to = w;
-    else if (j >= first) *to += w;
+    else *to += w;
 }
 
 // ---------------------------------------------------------------------------------------
-template <typename T, int DH> int launch_tree_dh(const TreeParams& P, int row_tiles, hipStream_t st) {
+template <typename T, int DH, int RT, int W> int launch_tree_kernel(const TreeParams& P, hipStream_t st) {
     const int pieces = P.B * P.H * P.n_splits;
-    const dim3 grid((unsigned)((pieces + 7) / 8 * 8 * P.row_blocks)), block(kTreeWaves * 64);
-    switch (row_tiles) {
-        case 1: hipLaunchKernelGGL((ffa_tree_kernel<T, DH, 1>), grid, block, 0, st, P); break;
-        case 2: hipLaunchKernelGGL((ffa_tree_kernel<T, DH, 2>), grid, block, 0, st, P); break;
-        default:
-            if constexpr (DH != 256) {
-                if (row_tiles == 3) hipLaunchKernelGGL((ffa_tree_kernel<T, DH, 3>), grid, block, 0, st, P);
-                else hipLaunchKernelGGL((ffa_tree_kernel<T, DH, 4>), grid, block, 0, st, P);
-                break;
-            }
-            return FFA_ERR_PLAN;
+    const dim3 grid((unsigned)((pieces + 7) / 8 * 8 * P.row_blocks));
+    const size_t lds = (size_t)(tree_merge_floats<DH, W>() + P.rows * P.score_lds) * sizeof(float);
+    hipLaunchKernelGGL((ffa_tree_kernel<T, DH, RT, W>), grid, dim3(W * 64), lds, st, P);
+    return hipGetLastError() == hipSuccess ? FFA_OK : FFA_ERR_LAUNCH;
+}
+
+template <typename T, int DH> int launch_tree_dh(const TreeParams& P, const TreePlan& plan, hipStream_t st) {
+    int rc = FFA_ERR_PLAN;
+    if (plan.waves > 4) {
+        if constexpr (DH != 256) {
+            constexpr int W = tree_wide_waves(DH, 1);
+            if (plan.row_tiles == 1 && plan.waves == W) rc = launch_tree_kernel<T, DH, 1, W>(P, st);
+        }
+        if constexpr (tree_wide_waves(DH, 2) != 0)
+            if (plan.row_tiles == 2 && plan.waves == tree_wide_waves(DH, 2)) rc = launch_tree_kernel<T, DH, 2, tree_wide_waves(DH, 2)>(P, st);
+    } else {
+        if (plan.row_tiles == 1) rc = launch_tree_kernel<T, DH, 1, 4>(P, st);
+        if (plan.row_tiles == 2) rc = launch_tree_kernel<T, DH, 2, 4>(P, st);
+        if constexpr (tree_row_tiles(DH) > 2)
+            if (plan.row_tiles == 3) rc = launch_tree_kernel<T, DH, 3, 4>(P, st);
+        if constexpr (tree_row_tiles(DH) > 3)
+            if (plan.row_tiles == 4) rc = launch_tree_kernel<T, DH, 4, 4>(P, st);
     }
-    if (hipGetLastError() != hipSuccess) return FFA_ERR_LAUNCH;
-    if (P.n_splits > 1) {
-        const long long threads = (long long)P.B * P.H * P.rows * (DH / 4);
-        hipLaunchKernelGGL((ffa_tree_join_kernel<T, DH>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, P);
-        if (hipGetLastError() != hipSuccess) return FFA_ERR_LAUNCH;
-    }
-    if (P.ws_scores != nullptr) {
-        const int blocks = (P.t + 1 + 255) / 256;
-        hipLaunchKernelGGL(ffa_tree_weights_kernel, dim3((unsigned)(P.B * P.H * blocks)), dim3(256), 0, st, P, blocks);
+    if (rc != FFA_OK) return rc;
+    const bool weights = P.ws_scores != nullptr && (P.n_splits > 1 || P.score_lds == 0);
+    if (P.n_splits > 1 || weights) {
+        const long long threads = P.n_splits > 1 ? (long long)P.B * P.H * P.rows * (DH / 4) : 0;
+        const int join_blocks = (int)((threads + 255) / 256), key_blocks = (P.t + 1 + 255) / 256;
+        const long long blocks = join_blocks + (weights ? (long long)P.B * P.H * key_blocks : 0);
+        if (blocks > 0x7fffffffll) return FFA_ERR_SHAPE;
+        hipLaunchKernelGGL((ffa_tree_finish_kernel<T, DH>), dim3((unsigned)blocks), dim3(256), 0, st, P, join_blocks, key_blocks);
         if (hipGetLastError() != hipSuccess) return FFA_ERR_LAUNCH;
     }
     return FFA_OK;
 }
 
-template <typename T> int launch_tree_type(const TreeParams& P, int head_dim, int row_tiles, void* stream) {
+template <typename T> int launch_tree_type(const TreeParams& P, int head_dim, const TreePlan& plan, void* stream) {
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     switch (head_dim) {
-        case 64: return launch_tree_dh<T, 64>(P, row_tiles, st);
-        case 80: return launch_tree_dh<T, 80>(P, row_tiles, st);
-        case 128: return launch_tree_dh<T, 128>(P, row_tiles, st);
-        case 256: return launch_tree_dh<T, 256>(P, row_tiles, st);
+        case 64: return launch_tree_dh<T, 64>(P, plan, st);
+        case 80: return launch_tree_dh<T, 80>(P, plan, st);
+        case 128: return launch_tree_dh<T, 128>(P, plan, st);
+        case 256: return launch_tree_dh<T, 256>(P, plan, st);
         default: return FFA_ERR_HEAD_DIM;
     }
 }
