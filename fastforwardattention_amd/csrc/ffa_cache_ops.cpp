@@ -12,6 +12,9 @@ using namespace ffa;
 
 namespace {
 
+// Most heads of a cache, and most query heads that share one of them.
+constexpr int kTreeHeads = 4096;
+
 bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
@@ -24,13 +27,14 @@ int check_cache_shape(int precision, int B, int H, int Dh, int Lmax) {
     if (elem_bytes(precision) == 0) return FFA_ERR_DTYPE;
     if (Dh != 64 && Dh != 80 && Dh != 128 && Dh != 256) return FFA_ERR_HEAD_DIM;
     if (B <= 0 || H <= 0 || Lmax <= 0) return FFA_ERR_SHAPE;
-    // Four chunk rows of a K cache are addressed with 32 bits from their first byte.
-    if ((long long)B * H > (1ll << 20) || Lmax > (1 << 25)) return FFA_ERR_SHAPE;
+    // Four chunk rows of a K cache are addressed with 32 bits from their first byte; pairs, heads and rows
+    // are divided by multiplication with 32-bit factors (tree_magic), and pairs / 8 is a grid's y.
+    if ((long long)B * H > (1ll << 18) || H > kTreeHeads || Lmax > (1 << 25)) return FFA_ERR_SHAPE;
     return FFA_OK;
 }
 
 // Weight-summing step: scores of the cached keys in whole wave tiles, the new token's behind them.
-int score_stride_of(int t) { return (int)align_up((size_t)t, 32) + 32; }
+int score_stride_of(int t) { return (int)align_up((size_t)t, 64) + 64; }
 
 struct TreeSizes {
     size_t acc = 0, ml = 0, scores = 0;
@@ -49,8 +53,11 @@ TreeSizes tree_sizes(int pairs, int rows, int head_dim, int n_splits, bool score
 // Scores of a piece are held in LDS, next to the merge buffer, up to this many words.
 constexpr int kScoreLdsWords = 16384;
 
+// Joining pieces costs a kernel, about 4 us: what 12 tiles take a workgroup (0.3 us a tile).
+constexpr int kJoinTiles = 12;
+
 struct TreeShape {
-    int row_tiles, row_blocks, waves, most_splits;
+    int row_tiles, row_blocks, tile_keys, most_splits;
 };
 
 // What does not depend on the cut of the keys.  most_splits grows with t.
@@ -59,14 +66,12 @@ TreeShape tree_shape(int precision, int pairs, int rows, int head_dim, int t, in
     const int row_tiles = ceil_div(rows, 16);
     s.row_blocks = ceil_div(row_tiles, tree_row_tiles(head_dim));
     s.row_tiles = ceil_div(row_tiles, s.row_blocks);
-    const int tiles = ceil_div(t, tree_tile_keys(precision));
-    const int wide = tree_wide_waves(head_dim, s.row_tiles);
+    s.tile_keys = 16 * tree_tile_units(elem_bytes(precision), head_dim, s.row_tiles);
+    const int tiles = ceil_div(t, s.tile_keys), groups = pairs * s.row_blocks;
     // One workgroup a CU streams at the memory's rate (measured from 1/4 to 16 a CU: 8 heads x 20000 keys
-    // 167, 95, 63, 84, 117 us at 1/4, 1/2, 1, 2, 4), more only add partial results to join.  Where pairs and
-    // row blocks are fewer than the CUs, workgroups have as many waves as a CU holds.
-    const int groups = pairs * s.row_blocks;
-    s.waves = wide != 0 && groups < cus ? wide : 4;
-    s.most_splits = std::max(1, std::min({ceil_div(cus, groups), tiles / (2 * s.waves), 128}));
+    // 167, 95, 63, 84, 117 us at 1/4, 1/2, 1, 2, 4), more only add partial results to join.
+    const int most = std::max(1, std::min({ceil_div(cus, groups), tiles / 2, 128}));
+    s.most_splits = tiles - tiles / most < kJoinTiles ? 1 : most;
     return s;
 }
 
@@ -90,6 +95,9 @@ int run_tree(int precision, int head_dim, TreeParams& P, void* workspace, size_t
     P.n_splits = plan.n_splits;
     P.tiles_per_split = plan.tiles_per_split;
     P.row_blocks = plan.row_blocks;
+    P.splits_magic = tree_magic(P.n_splits);
+    P.H_magic = tree_magic(P.H);
+    P.G_magic = tree_magic(P.G);
     return launch_tree(precision, head_dim, P, plan, stream);
 }
 
@@ -129,11 +137,14 @@ TreePlan plan_tree(int precision, int pairs, int rows, int head_dim, int t, bool
     TreePlan p;
     p.row_tiles = shape.row_tiles;
     p.row_blocks = shape.row_blocks;
-    p.waves = shape.waves;
-    const int tile = tree_tile_keys(precision), tiles = ceil_div(t, tile);
+    const int tile = shape.tile_keys, tiles = ceil_div(t, tile);
     p.tiles_per_split = std::max(1, ceil_div(tiles, shape.most_splits));
     p.n_splits = std::max(1, ceil_div(tiles, p.tiles_per_split));
-    const long long words = (long long)p.tiles_per_split * tile + 32;
+    // With one workgroup a CU at most, 8 waves where they have two tiles each (256 pairs, 8000 keys, 32 rows
+    // 109 -> 81 us, 64 rows 123 -> 102 us); more workgroups share the CUs, and 8 waves would not fit twice
+    // (320 pairs, 1128 keys, 32 rows 27 -> 33 us).
+    p.waves = tree_wide(head_dim, p.row_tiles) && pairs * p.row_blocks * p.n_splits <= cus && p.tiles_per_split >= 16 ? 8 : 4;
+    const long long words = (long long)p.tiles_per_split * tile + 64;
     p.score_lds = weights && rows <= 16 && words * rows <= kScoreLdsWords ? (int)words : 0;
     return p;
 }
@@ -160,12 +171,14 @@ int ffa_attention_tree(int precision, int batch_size, int head_num, int head_dim
     if (!tokens || !q || !k || !v || !k_cache || !v_cache || !out) return FFA_ERR_NULL_POINTER;
     const int n = tokens->tokens, Hq = tokens->q_head_num;
     if (n < 1 || n > FFA_MAX_TREE_TOKENS || n > max_seq_len - t || Hq <= 0 || Hq % head_num != 0) return FFA_ERR_TREE;
-    if ((long long)batch_size * Hq * n > (1ll << 24)) return FFA_ERR_SHAPE;
+    if ((long long)batch_size * Hq * n > (1ll << 24) || Hq / head_num > kTreeHeads) return FFA_ERR_SHAPE;
     const int unit = 16 / elem_bytes(precision);
     for (int i = 0; i < 3; ++i)
         if (tokens->q_stride[i] % unit || tokens->k_stride[i] % unit || tokens->v_stride[i] % unit ||
             tokens->out_stride[i] % unit)
             return FFA_ERR_TREE;
+    for (long long step : {tokens->k_stride[2], tokens->v_stride[2]})  // lanes count rows in 32 bits
+        if (step < 0 || step >= (1 << 26) / elem_bytes(precision)) return FFA_ERR_TREE;
     for (const void* p : {q, k, v, (const void*)k_cache, (const void*)v_cache, (const void*)out})
         if (!aligned(p, 16)) return FFA_ERR_ALIGNMENT;
     for (const int32_t* p : {tokens->parents, tokens->first_keys, tokens->lengths, tokens->counts})
@@ -194,7 +207,7 @@ int ffa_attention_weights(int precision, int batch_size, int head_num, int q_hea
     if (t < 0 || t >= max_seq_len) return FFA_ERR_TIMESTEP;
     if (!q || !k || !v || !k_cache || !v_cache || !out || !key_weights) return FFA_ERR_NULL_POINTER;
     if (q_head_num <= 0 || q_head_num % head_num != 0) return FFA_ERR_TREE;
-    if ((long long)batch_size * q_head_num > (1ll << 24)) return FFA_ERR_SHAPE;
+    if ((long long)batch_size * q_head_num > (1ll << 24) || q_head_num / head_num > kTreeHeads) return FFA_ERR_SHAPE;
     for (const void* p : {q, k, v, (const void*)k_cache, (const void*)v_cache, (const void*)out})
         if (!aligned(p, 16)) return FFA_ERR_ALIGNMENT;
     if (!aligned(key_weights, 4) || !aligned(first_keys, 4) || !aligned(lengths, 4)) return FFA_ERR_ALIGNMENT;

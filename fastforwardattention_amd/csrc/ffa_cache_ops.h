@@ -14,22 +14,25 @@ namespace ffa {
 // its G query heads, row = token * G + head -- are cut into blocks of row_tiles * 16; a workgroup
 // takes one row block over one piece of the keys, its waves every n-th tile of them.
 
-// Keys of one wave tile: two (16-bit) or one (fp32) matrix tiles of 16 keys.
-inline int tree_tile_keys(int precision) { return precision == FFA_PRECISION_F32 ? 16 : 32; }
+// 16-key matrix tiles of a wave tile: 32 keys (16 in fp32) are what one product over keys takes; with
+// one row tile and narrow heads the registers hold twice that, and a wave has twice the loads in flight.
+constexpr int tree_tile_units(int elem_bytes, int head_dim, int row_tiles) {
+    return (elem_bytes == 2 ? 2 : 1) * (row_tiles == 1 && head_dim <= 80 ? 2 : 1);
+}
 
 // Most 16-row matrix tiles a wave holds without spilling registers.
-constexpr int tree_row_tiles(int head_dim) { return head_dim == 256 ? 2 : head_dim == 128 ? 3 : 4; }
+constexpr int tree_row_tiles(int head_dim) { return head_dim == 256 ? 1 : 4; }
 
-// Waves of a workgroup where the pairs alone do not fill the chip: what the registers of the kernel
-// let a CU hold (0: no such kernel).  Elsewhere workgroups have 4.
-constexpr int tree_wide_waves(int head_dim, int row_tiles) {
-    return head_dim == 64 && row_tiles == 1 ? 16 : head_dim * row_tiles <= 128 ? 8 : 0;
-}
+// Whether two waves a SIMD fit the registers.
+constexpr bool tree_two_waves(int head_dim, int row_tiles) { return head_dim <= 128 && head_dim * row_tiles <= 256; }
+// Whether there is a kernel of 8 waves beside the one of 4: where a wave's loads are too few for 4 of
+// them to keep a CU's share of the memory busy.
+constexpr bool tree_wide(int head_dim, int row_tiles) { return tree_two_waves(head_dim, row_tiles) && !(head_dim == 128 && row_tiles == 2); }
 
 struct TreePlan {
     int row_tiles;        // 16-row matrix tiles a wave holds: 1 .. 4
     int row_blocks;       // workgroups a piece of keys is read by
-    int waves;            // of a workgroup: 4, or tree_wide_waves()
+    int waves;            // of a workgroup: 4, or 8 (tree_wide)
     int n_splits;         // pieces of the cached keys
     int tiles_per_split;  // wave tiles a piece holds
     int score_lds;        // weight-summing step: words of a row of scores held in LDS, 0 = in the workspace
@@ -50,7 +53,11 @@ struct TreeParams {
     float scale_log2e;  // |softmax_scale| * log2(e), never zero
     int q_sign;         // sign of softmax_scale: Q enters with it
     int n_splits, tiles_per_split, row_blocks;
+    unsigned splits_magic, H_magic, G_magic;  // tree_magic() of n_splits, H and G
 };
+
+// n / d = (n * tree_magic(d)) >> 32 while n * d < 2^32 (d > 1).
+inline unsigned tree_magic(int d) { return d > 1 ? (unsigned)(0x100000000ull / (unsigned)d) + 1u : 0u; }
 
 TreePlan plan_tree(int precision, int pairs, int rows, int head_dim, int t, bool weights, int cus);
 int launch_tree(int precision, int head_dim, const TreeParams& P, const TreePlan& plan, void* stream);

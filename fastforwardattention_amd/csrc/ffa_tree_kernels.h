@@ -37,12 +37,12 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 // row's largest is still above half the smallest number.
 constexpr float kSlack = 15.f, kLift = 6.f;
 
-// Geometry of one element type and head dimension.
-template <typename T, int DH> struct TreeGeo {
+// Geometry of one element type, head dimension and number of row tiles.
+template <typename T, int DH, int RT> struct TreeGeo {
     static constexpr int X = Elem<T>::X;                 // elements of a 16-byte chunk
     static constexpr int NCH = DH / X;                   // chunks of a row
     static constexpr int KK = (NCH + 3) / 4;             // chunk groups of a K row, one chunk a lane group
-    static constexpr int NU = X == 8 ? 2 : 1;            // 16-key matrix tiles of a wave tile
+    static constexpr int NU = tree_tile_units(sizeof(T), DH, RT);  // 16-key matrix tiles of a wave tile
     static constexpr int TK = 16 * NU;                   // keys of a wave tile
     // A V row is cut into blocks of 16 * E dims, E of them a lane: E = 8 or 4 (16 or 8 bytes), the
     // last 16 dims of Dh = 80 one by one.
@@ -90,7 +90,7 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint3
     *lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, rest), tiny));
 }
 
-template <typename T> __device__ __forceinline__ PFrag16 split_weights(const float (&p)[8], T tag) {
+template <typename T> __device__ __forceinline__ PFrag16 split_weights(const float* p, T tag) {
     PFrag16 f;
     split_pair(p[0], p[1], &f.hi.x, &f.lo.x, tag);
     split_pair(p[2], p[3], &f.hi.y, &f.lo.y, tag);
@@ -101,8 +101,8 @@ template <typename T> __device__ __forceinline__ PFrag16 split_weights(const flo
 
 // ---------------------------------------------------------------------------------------
 // V pieces of one wave tile, as loaded: piece j of a lane belongs to key 16 (j / 4) + 4 g + j % 4.
-template <typename T, int DH> struct VTile {
-    using G = TreeGeo<T, DH>;
+template <typename T, int DH, int RT> struct VTile {
+    using G = TreeGeo<T, DH, RT>;
     static constexpr int NJ = 4 * G::NU;
     static constexpr int WORDS = G::E * (int)sizeof(T) / 4;     // 32-bit words of a piece: 2 or 4
     uint32_t w[NJ][G::NBLK][WORDS];
@@ -135,35 +135,56 @@ template <typename T, int DH> struct VTile {
             for (int i = 0; i < WORDS; ++i) w[j][b][i] = 0;
         if constexpr (G::TAIL != 0) tail[j] = 0;
     }
-    // Infinities and NaN of key j become zero; true if there was one.
-    __device__ __forceinline__ bool drop_nonfinite(int j) {
-        bool any = false;
-        auto word = [&](uint32_t x) -> uint32_t {
-            if constexpr (sizeof(T) == 4) {
-                const bool bad = (x & 0x7f800000u) == 0x7f800000u;
-                any |= bad;
-                return bad ? 0u : x;
-            } else {
-                constexpr uint32_t e = __is_same(T, bf16_t) ? 0x7f80u : 0x7c00u;
-                const bool lo = (x & e) == e, hi = ((x >> 16) & e) == e;
-                any |= lo | hi;
-                return x & (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu);
-            }
+    // Whether key j holds an infinity or NaN: the exponent's bits are all ones.
+    static constexpr uint32_t kExponent = sizeof(T) == 4 ? 0x7f800000u : __is_same(T, bf16_t) ? 0x7f80u : 0x7c00u;
+    __device__ __forceinline__ bool nonfinite(int j) const {
+        uint32_t top = 0;  // largest magnitude; of both halves in 16-bit types
+        auto word = [&](uint32_t x) {
+            if constexpr (sizeof(T) == 4) top = max(top, x & 0x7fffffffu);
+            else top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, top), __builtin_bit_cast(u16x2_t, x & 0x7fff7fffu)));
+        };
+#pragma unroll
+        for (int b = 0; b < G::NBLK; ++b)
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) word(w[j][b][i]);
+        if constexpr (G::TAIL != 0) word(tail[j]);
+        if constexpr (sizeof(T) == 4) return top >= kExponent;
+        else return (top & 0xffffu) >= kExponent || (top >> 16) >= kExponent;
+    }
+    // Infinities and NaN of key j become zero.
+    __device__ __forceinline__ void drop_nonfinite(int j) {
+        auto word = [](uint32_t x) -> uint32_t {
+            if constexpr (sizeof(T) == 4) return (x & kExponent) == kExponent ? 0u : x;
+            else return x & ((x & kExponent) == kExponent ? 0xffff0000u : 0xffffffffu) &
+                        (((x >> 16) & kExponent) == kExponent ? 0x0000ffffu : 0xffffffffu);
         };
 #pragma unroll
         for (int b = 0; b < G::NBLK; ++b)
 #pragma unroll
             for (int i = 0; i < WORDS; ++i) w[j][b][i] = word(w[j][b][i]);
         if constexpr (G::TAIL != 0) tail[j] = word(tail[j]);
-        return any;
     }
-    // Left operand of result tile (block b, element e): 8 keys of dim b * 16 E + c * E + e.
-    __device__ __forceinline__ uint4 turned(int b, int e) const {
+    // Key j's pieces back to a row.
+    __device__ __forceinline__ void store(int j, char* row, int c) const {
+#pragma unroll
+        for (int b = 0; b < G::NBLK; ++b) {
+            char* p = row + (b * 16 + c) * (WORDS * 4);
+            if constexpr (WORDS == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[j][b][0], w[j][b][1], w[j][b][2], w[j][b][3]);
+            else *reinterpret_cast<uint2*>(p) = make_uint2(w[j][b][0], w[j][b][1]);
+        }
+        if constexpr (G::TAIL != 0) {
+            char* p = row + (G::NBLK * 16 * G::E + c) * (int)sizeof(T);
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(p) = tail[j];
+            else *reinterpret_cast<uint16_t*>(p) = (uint16_t)tail[j];
+        }
+    }
+    // Left operand of result tile (block b, element e): keys 8 i .. 8 i + 7 of dim b * 16 E + c * E + e.
+    __device__ __forceinline__ uint4 turned(int i, int b, int e) const {
         uint32_t o[4];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-            if (b < G::NBLK) o[p] = __builtin_amdgcn_perm(w[2 * p + 1][b][e / 2], w[2 * p][b][e / 2], e % 2 ? 0x07060302 : 0x05040100);
-            else o[p] = __builtin_amdgcn_perm(tail[G::TAIL ? 2 * p + 1 : 0], tail[G::TAIL ? 2 * p : 0], 0x05040100);
+            if (b < G::NBLK) o[p] = __builtin_amdgcn_perm(w[8 * i + 2 * p + 1][b][e / 2], w[8 * i + 2 * p][b][e / 2], e % 2 ? 0x07060302 : 0x05040100);
+            else o[p] = __builtin_amdgcn_perm(tail[G::TAIL ? 8 * i + 2 * p + 1 : 0], tail[G::TAIL ? 8 * i + 2 * p : 0], 0x05040100);
         }
         return make_uint4(o[0], o[1], o[2], o[3]);
     }
@@ -171,13 +192,6 @@ template <typename T, int DH> struct VTile {
         return __builtin_bit_cast(float, b < G::NBLK ? w[j][b][e] : tail[G::TAIL ? j : 0]);
     }
 };
-
-// Dim of result tile `db`, result row i (0 .. 15).
-template <typename T, int DH> __device__ __forceinline__ int tile_dim(int db, int i) {
-    using G = TreeGeo<T, DH>;
-    if (db < G::NBLK * G::E) return (db / G::E) * 16 * G::E + i * G::E + db % G::E;
-    return G::NBLK * 16 * G::E + i;
-}
 
 template <typename T> __device__ __forceinline__ float load_elem(const T* p);
 template <> __device__ __forceinline__ float load_elem(const uint16_t* p) { return (float)__builtin_bit_cast(_Float16, *p); }
@@ -194,6 +208,9 @@ __device__ __forceinline__ void store_out4(bf16_t* to, const f32x4_t& o) {
     *reinterpret_cast<u16x4_t*>(to) = u16x4_t{float_to_bf16(o[0]), float_to_bf16(o[1]), float_to_bf16(o[2]), float_to_bf16(o[3])};
 }
 __device__ __forceinline__ void store_out4(float* to, const f32x4_t& o) { *reinterpret_cast<f32x4_t*>(to) = o; }
+
+// n / d by the factor tree_magic(d).
+__device__ __forceinline__ int quotient(int n, int d, unsigned magic) { return d == 1 ? n : (int)__umulhi((unsigned)n, magic); }
 
 // Slots of sample b: [first, length).
 __device__ __forceinline__ void sample_range(const int* first_keys, const int* lengths, int b, int t, int* first, int* length) {
@@ -224,117 +241,131 @@ __device__ __forceinline__ uint64_t ancestor_mask(const int* parents, int tokens
 // ---------------------------------------------------------------------------------------
 // Waves a SIMD that the registers are cut for.  Two hide a wave's loads and transcendentals behind the
 // other's matrix products; what holds more than 256 registers of results and operands runs alone.
-constexpr int tree_waves_per_simd(int dh, int rt, int w) { return w > 4 ? w / 4 : dh <= 128 && dh * rt <= 256 ? 2 : 1; }
+constexpr int tree_waves_per_simd(int dh, int rt) { return tree_two_waves(dh, rt) ? 2 : 1; }
 
 // Floats of LDS in front of the scores: the waves' results of one row tile.
-template <int DH, int W> constexpr int tree_merge_floats() { return W * 16 * (DH + 4); }
+template <int DH, int W> constexpr int tree_merge_floats() { return W * 16 * DH; }
+
+// Arguments that the first loads need, ahead of the struct: they arrive in registers with the wave.
+#define TREE_HOT_DECL const char *k_cache, const char *v_cache, int Lmax, int t, int n_splits, unsigned splits_magic, \
+                      int tiles_per_split, int pieces, int ragged
+#define TREE_HOT_OF(P) static_cast<const char*>((P).k_cache), static_cast<const char*>((P).v_cache), (P).Lmax, (P).t, \
+                       (P).n_splits, (P).splits_magic, (P).tiles_per_split, (P).B * (P).H * (P).n_splits, \
+                       (int)((P).lengths != nullptr || (P).first_keys != nullptr)
 
 template <typename T, int DH, int RT, int W>
-__global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT, W)) ffa_tree_kernel(const TreeParams P) {
-    using G = TreeGeo<T, DH>;
+__global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT)) ffa_tree_kernel(TREE_HOT_DECL, const TreeParams P) {
+    using G = TreeGeo<T, DH, RT>;
     constexpr int NU = G::NU, TK = G::TK, KK = G::KK, NCH = G::NCH, DB = G::DB, NJ = 4 * NU;
-    constexpr int RS = DH + 4;  // floats of a row in the merge buffer
+    constexpr unsigned ROW = DH * sizeof(T);  // bytes of a cache row
+    constexpr bool SHORT = RT == 1;           // few new tokens are likely: skip 16 keys that hold none
     extern __shared__ float4 s_dynamic[];
-    float* const s_acc = reinterpret_cast<float*>(s_dynamic);     // [W][16 * RS]
-    float* const s_scores = s_acc + tree_merge_floats<DH, W>();   // [rows][score_lds], weight-summing step
-    __shared__ float s_ml[W][RT * 16][2];
-    __shared__ float s_row[16][2];  // weight-summing step: -M and 1 / L of a row
+    f32x4_t* const s_acc = reinterpret_cast<f32x4_t*>(s_dynamic);                               // [W][DB][64]
+    float* const s_scores = reinterpret_cast<float*>(s_dynamic) + tree_merge_floats<DH, W>();   // [rows][score_lds]
+    __shared__ float s_ml[W][RT * 16][2];  // a wave's m and l of a row; then s_ml[..][0] = its factor
+    __shared__ float s_row[RT * 16][2];    // M and L of a row
     __shared__ uint64_t s_seen[64];
-    __shared__ unsigned s_bad[2];
+    __shared__ uint64_t s_bad[64 / TK];
 
     // Row blocks of one piece are 8 workgroups apart: the same XCD, whose L2 then holds the piece.
-    const int span = 8 * P.row_blocks;
-    const int octet = blockIdx.x / span, in = blockIdx.x % span;
-    const int rb = in / 8, piece = octet * 8 + in % 8;
-    const int pairs = P.B * P.H;
-    if (piece >= pairs * P.n_splits) return;
-    const int pair = piece / P.n_splits, split = piece % P.n_splits;
-    const int b = pair / P.H, h = pair % P.H;
+    const int rb = blockIdx.x / 8, piece = blockIdx.y * 8 + blockIdx.x % 8;
+    if (piece >= pieces) return;
+    const int pair = quotient(piece, n_splits, splits_magic), split = piece - pair * n_splits;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, c = lane & 15;
+    const char* kc = k_cache + (size_t)pair * (unsigned)Lmax * ROW;
+    const char* vc = v_cache + (size_t)pair * (unsigned)Lmax * ROW;
 
-    int first, length;
-    sample_range(P.first_keys, P.lengths, b, P.t, &first, &length);
-    const int count = P.counts ? min(max(P.counts[b], 0), P.tokens) : P.tokens;
-    const bool last = split == P.n_splits - 1;
-    const size_t cache_row = (size_t)DH * sizeof(T);
-    const char* kc = static_cast<const char*>(P.k_cache) + (size_t)pair * P.Lmax * cache_row;
-    const char* vc = static_cast<const char*>(P.v_cache) + (size_t)pair * P.Lmax * cache_row;
-    const char* kn = static_cast<const char*>(P.k) + (b * P.k_stride[0] + h * P.k_stride[1]) * (long long)sizeof(T);
-    const char* vn = static_cast<const char*>(P.v) + (b * P.v_stride[0] + h * P.v_stride[1]) * (long long)sizeof(T);
-    const long long kn_row = P.k_stride[2] * (long long)sizeof(T), vn_row = P.v_stride[2] * (long long)sizeof(T);
-    const int row0 = rb * RT * 16;
+    int first = 0, length = t;
+    if (ragged) sample_range(P.first_keys, P.lengths, quotient(pair, P.H, P.H_magic), t, &first, &length);
 
     // This wave's tiles: wave, wave + W, ... of the piece's cached keys, then its share of the tiles
     // of new tokens, which are dealt from the last wave on (the piece's shorter ends).
-    const int piece0 = split * P.tiles_per_split * TK;
-    const int lo = max(split * P.tiles_per_split, first / TK) + wave;
-    const int hi = min((split + 1) * P.tiles_per_split, (length + TK - 1) / TK);
+    const int piece0 = split * tiles_per_split * TK;
+    const int lo = max(split * tiles_per_split, first / TK) + wave;
+    const int hi = min((split + 1) * tiles_per_split, (length + TK - 1) / TK);
     const int n_cached = max(0, (hi - lo + W - 1) / W);
-    const int n_new = last ? max(0, ((count + TK - 1) / TK + wave) / W) : 0;
-    const int n_tiles = n_cached + n_new;
 
     uint4 kf[NU][KK];
-    VTile<T, DH> vt;
+    VTile<T, DH, RT> vt;
     // A chunk that does not exist (Dh = 80) must not hold an infinity against the zero of Q.
     auto existing = [&](const uint4& x, int kk) {
         if (NCH % 4 != 0 && kk == KK - 1 && kk * 4 + g >= NCH) return make_uint4(0, 0, 0, 0);
         return x;
     };
+    // Loads of a tile: uniform addresses plus a 32-bit offset a lane.  Rows past `most` are read from it,
+    // and masked.  In V of a whole tile of cached keys the rows are compile-time distances apart.
+    auto load_cached_k = [&](int key0, int most) {
+        const char* base = kc + (size_t)key0 * 16;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            const int gg = NCH % 4 != 0 && kk == KK - 1 ? min(g, NCH - 1 - kk * 4) : g;
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+                kf[u][kk] = existing(ld16(base + (size_t)kk * 4 * (unsigned)Lmax * 16 +
+                                          ((unsigned)gg * (unsigned)Lmax + (unsigned)min(u * 16 + c, most)) * 16u), kk);
+        }
+    };
+    auto load_whole_v = [&](int key0) {
+        const char* base = vc + (size_t)key0 * ROW;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) vt.load(j, base + ((j / 4) * 16 + j % 4) * ROW, (unsigned)g * 4u * ROW, c);
+    };
+    auto load_rows_v = [&](const char* base, unsigned step, int most) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+            if (!SHORT || j / 4 * 16 <= most) vt.load(j, base, (unsigned)min((j / 4) * 16 + g * 4 + j % 4, most) * step, c);
+    };
+    const bool begun = n_cached > 0 && lo * TK + TK <= length;
+    if (begun) {
+        load_cached_k(lo * TK, TK);
+        load_whole_v(lo * TK);
+    }
+
+    // What the rest of the arguments say.
+    const int b = quotient(pair, P.H, P.H_magic), h = pair - b * P.H;
+    const int count = P.counts ? min(max(P.counts[b], 0), P.tokens) : P.tokens;
+    const bool last = split == n_splits - 1;
+    const char* kn = static_cast<const char*>(P.k) + (b * P.k_stride[0] + h * P.k_stride[1]) * (long long)sizeof(T);
+    const char* vn = static_cast<const char*>(P.v) + (b * P.v_stride[0] + h * P.v_stride[1]) * (long long)sizeof(T);
+    const unsigned kn_row = (unsigned)P.k_stride[2] * (unsigned)sizeof(T), vn_row = (unsigned)P.v_stride[2] * (unsigned)sizeof(T);
+    const int row0 = rb * RT * 16;
+    const int n_new = last ? max(0, ((count + TK - 1) / TK + wave) / W) : 0;
+    const int n_tiles = n_cached + n_new;
     // Tile i of this wave: its first key, counted in the cache or among the new tokens.
     auto key0_of = [&](int i) { return (i < n_cached ? lo + i * W : W - 1 - wave + (i - n_cached) * W) * TK; };
-    // A whole tile of cached keys: uniform addresses plus one fixed offset a lane.  Any other tile:
-    // rows past the end are read from the last one, and masked.
-    const unsigned k_lane = ((unsigned)g * (unsigned)P.Lmax + (unsigned)c) * 16u;
-    const unsigned k_lane_end = ((unsigned)min(g, NCH - 1 - (KK - 1) * 4) * (unsigned)P.Lmax + (unsigned)c) * 16u;
-    const unsigned v_lane = (unsigned)g * 4u * (unsigned)cache_row;
-    auto whole_tile = [&](int i) { return i < n_cached && key0_of(i) + TK <= length; };
     auto load_k = [&](int i) {
         const int key0 = key0_of(i);
-        if (whole_tile(i)) {
-            const char* base = kc + (size_t)key0 * 16;
-#pragma unroll
-            for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-                for (int u = 0; u < NU; ++u) {
-                    const char* from = base + (size_t)kk * 4 * P.Lmax * 16 + u * 256;
-                    kf[u][kk] = existing(ld16(from + (NCH % 4 != 0 && kk == KK - 1 ? k_lane_end : k_lane)), kk);
-                }
+        if (i < n_cached) {
+            load_cached_k(key0, length - 1 - key0);
         } else {
-            const bool cached = i < n_cached;
-            const char* base = cached ? kc : kn;
-            const long long row_step = cached ? 16 : kn_row, chunk_step = cached ? (long long)P.Lmax * 16 : 16;
-            const int end = (cached ? length : count) - 1;
+            const char* base = kn + (size_t)key0 * kn_row;
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
-                const char* row = base + min(key0 + u * 16 + c, end) * row_step;
+                if (SHORT && key0 + u * 16 >= count) break;
+                const unsigned row = (unsigned)min(u * 16 + c, count - 1 - key0) * kn_row;
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk) kf[u][kk] = existing(ld16(row + min(kk * 4 + g, NCH - 1) * chunk_step), kk);
+                for (int kk = 0; kk < KK; ++kk) kf[u][kk] = existing(ld16(base + (row + (unsigned)min(kk * 4 + g, NCH - 1) * 16u)), kk);
             }
         }
     };
     auto load_v = [&](int i) {
         const int key0 = key0_of(i);
-        if (whole_tile(i)) {
-            const char* base = vc + (size_t)key0 * cache_row;
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) vt.load(j, base + ((j / 4) * 16 + j % 4) * cache_row, v_lane, c);
-        } else {
-            const bool cached = i < n_cached;
-            const char* base = cached ? vc : vn;
-            const long long step = cached ? (long long)cache_row : vn_row;
-            const int end = (cached ? length : count) - 1;
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) vt.load(j, base + min(key0 + (j / 4) * 16 + g * 4 + j % 4, end) * step, 0u, c);
-        }
+        if (i < n_cached && key0 + TK <= length) load_whole_v(key0);
+        else if (i < n_cached) load_rows_v(vc + (size_t)key0 * ROW, ROW, length - 1 - key0);
+        else load_rows_v(vn + (size_t)key0 * vn_row, vn_row, count - 1 - key0);
     };
-    if (n_tiles > 0) {
+    if (!begun && n_tiles > 0) {
         load_k(0);
         load_v(0);
     }
 
-    if (tid < 2) s_bad[tid] = 0;
-    if (last && wave == 0) s_seen[lane] = ancestor_mask(P.parents ? P.parents + (size_t)b * P.tokens : nullptr, P.tokens, lane);
+    // Lane i of a wave that has new tokens: node i's ancestors.
+    uint64_t ancestors = 0;
+    if (n_new > 0) {
+        ancestors = ancestor_mask(P.parents ? P.parents + (size_t)b * P.tokens : nullptr, P.tokens, lane);
+        if (wave == W - 1) s_seen[lane] = ancestors;
+    }
 
     // Q: chunk kk * 4 + g of row row0 + rt * 16 + c; rows and chunks that do not exist are zero.
     // The factor of the scores is positive: a negative softmax_scale turns Q's sign.
@@ -342,7 +373,7 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT, W)) ffa_tr
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const int row = row0 + rt * 16 + c;
-        const int token = row / P.G, gh = row % P.G;
+        const int token = quotient(row, P.G, P.G_magic), gh = row - token * P.G;
         const char* qr = static_cast<const char*>(P.q) +
                          (b * P.q_stride[0] + (long long)(h * P.G + gh) * P.q_stride[1] + token * P.q_stride[2]) * (long long)sizeof(T);
 #pragma unroll
@@ -358,7 +389,6 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT, W)) ffa_tr
             }
         }
     }
-    __syncthreads();
 
     f32x4_t acc[RT][DB];
     float m[RT], l[RT];
@@ -374,6 +404,26 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT, W)) ffa_tr
         const int key0 = key0_of(i);
         const bool cached = i < n_cached;
         const bool masked = !cached || key0 < first || key0 + TK > length;
+        // New tokens are appended from the registers that hold them; nobody reads cache slots from
+        // `length` on.
+        if (!cached && rb == 0) {
+            char* kw = const_cast<char*>(kc);
+            char* vw = const_cast<char*>(vc);
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                if (SHORT && key0 + u * 16 >= count) break;
+                const int node = key0 + u * 16 + c;
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk)
+                    if (node < count && kk * 4 + g < NCH) st16(kw + ((size_t)(kk * 4 + g) * Lmax + length + node) * 16, kf[u][kk]);
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                if (SHORT && key0 + j / 4 * 16 >= count) break;
+                const int node = key0 + (j / 4) * 16 + g * 4 + j % 4;
+                if (node < count) vt.store(j, vw + (size_t)(length + node) * ROW, c);
+            }
+        }
         f32x4_t s[RT][NU];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -387,20 +437,25 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT, W)) ffa_tr
         if (masked) {
             // Bit j: this lane's key j is seen.  Cached keys: the sample's range; new ones: ancestors.
             auto bits_of = [&](uint64_t range) {
-                uint32_t x = (uint32_t)(range >> (g * 4)) & 15u;
-                if (NU == 2) x |= ((uint32_t)(range >> (16 + g * 4)) & 15u) << 4;
+                uint32_t x = 0;
+#pragma unroll
+                for (int u = 0; u < NU; ++u) x |= ((uint32_t)(range >> (u * 16 + g * 4)) & 15u) << (4 * u);
                 return x;
             };
             uint64_t range = 0;
             if (cached) {
-                const int from = max(first - key0, 0), to = min(length - key0, TK);
-                range = ((1ull << to) - 1) & ~((1ull << from) - 1);
+                const int from = min(max(first - key0, 0), TK), to = min(length - key0, TK);
+                range = (to == 64 ? ~0ull : (1ull << to) - 1) & (from == 64 ? 0ull : ~0ull << from);
             }
             uint32_t held = cached ? bits_of(range) : 0;
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                const int row = row0 + rt * 16 + c;
-                const uint32_t bits = cached ? held : row < P.rows ? bits_of(s_seen[row / P.G] >> key0) : 0u;
+                uint32_t bits = held;
+                if (!cached) {
+                    const int row = row0 + rt * 16 + c, token = min(quotient(row, P.G, P.G_magic), 63);
+                    const uint64_t of_row = (uint64_t)(uint32_t)__shfl((int)(ancestors >> 32), token) << 32 | (uint32_t)__shfl((int)ancestors, token);
+                    bits = row < P.rows ? bits_of(of_row >> key0) : 0u;
+                }
 #pragma unroll
                 for (int j = 0; j < NJ; ++j)
                     if (!(bits >> j & 1)) s[rt][j / 4][j % 4] = -INFINITY;
@@ -412,30 +467,49 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT, W)) ffa_tr
                 for (int j = 0; j < NJ; ++j)
                     if (!(held >> j & 1)) vt.clear(j);
             } else {
+                bool any = false;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
-                    const int node = key0 + (j / 4) * 16 + g * 4 + j % 4;
-                    if (node >= count) vt.clear(j);
-                    else if (vt.drop_nonfinite(j)) atomicOr(&s_bad[node / 32], 1u << (node % 32));
+                    if (key0 + (j / 4) * 16 + g * 4 + j % 4 >= count) vt.clear(j);
+                    if (!SHORT || key0 + j / 4 * 16 < count) any |= vt.nonfinite(j);
                 }
+                uint64_t bad = 0;
+                if (__any(any)) {
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        const uint64_t who = __ballot(vt.nonfinite(j));
+                        vt.drop_nonfinite(j);
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) bad |= (who >> (16 * w) & 0xffff) != 0 ? 1ull << ((j / 4) * 16 + w * 4 + j % 4) : 0ull;
+                    }
+                }
+                if (lane == 0) s_bad[key0 / TK] = bad;
             }
         }
         if (P.ws_scores != nullptr) {
             // In LDS if the piece's fit (key - first key of the piece), else in the workspace; the new
-            // token's scores lie in the last 32 words.
+            // token's scores lie in the last 64 words.
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 const int row = row0 + rt * 16 + c;
                 if (row < P.rows) {
-                    float* to = P.score_lds != 0
-                                    ? s_scores + row * P.score_lds + (cached ? key0 - piece0 : P.score_lds - 32)
-                                    : P.ws_scores + ((size_t)pair * P.rows + row) * P.score_stride + (cached ? key0 : P.score_stride - 32);
+                    f32x4_t x[NU];
 #pragma unroll
-                    for (int u = 0; u < NU; ++u) *reinterpret_cast<f32x4_t*>(to + g * 4 + u * 16) = s[rt][u] * P.scale_log2e;
+                    for (int u = 0; u < NU; ++u) x[u] = s[rt][u] * P.scale_log2e;
+                    if (P.score_lds != 0) {
+                        float* to = s_scores + row * P.score_lds + (cached ? key0 - piece0 : P.score_lds - 64) + g * 4;
+#pragma unroll
+                        for (int u = 0; u < NU; ++u) *reinterpret_cast<f32x4_t*>(to + u * 16) = x[u];
+                    } else {
+                        float* to = P.ws_scores + ((size_t)pair * P.rows + row) * P.score_stride + (cached ? key0 : P.score_stride - 64) + g * 4;
+#pragma unroll
+                        for (int u = 0; u < NU; ++u) *reinterpret_cast<f32x4_t*>(to + u * 16) = x[u];
+                    }
                 }
             }
         }
-        PFrag16 pf[RT];
+        constexpr int NP = sizeof(T) == 2 ? NU / 2 : 1;  // right operands of 32 keys
+        PFrag16 pf[RT][NP];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             float x[NJ];
@@ -462,34 +536,53 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT, W)) ffa_tr
             }
             l[rt] += sum;
             if constexpr (sizeof(T) == 2) {
-                pf[rt] = split_weights(x, T{});
+#pragma unroll
+                for (int q = 0; q < NP; ++q) pf[rt][q] = split_weights(x + 8 * q, T{});
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s[rt][0][j] = x[j];
+                for (int j = 0; j < NJ; ++j) s[rt][j / 4][j % 4] = x[j];
             }
         }
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
             const int blk = db < G::NBLK * G::E ? db / G::E : G::NBLK, e = db < G::NBLK * G::E ? db % G::E : 0;
             if constexpr (sizeof(T) == 2) {
-                const uint4 a = vt.turned(blk, e);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    acc[rt][db] = mma_qk(a, pf[rt].hi, acc[rt][db], T{});
-                    acc[rt][db] = mma_qk(a, pf[rt].lo, acc[rt][db], T{});
+                for (int q = 0; q < NP; ++q) {
+                    const uint4 a = vt.turned(q, blk, e);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        acc[rt][db] = mma_qk(a, pf[rt][q].hi, acc[rt][db], T{});
+                        acc[rt][db] = mma_qk(a, pf[rt][q].lo, acc[rt][db], T{});
+                    }
                 }
             } else {
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[rt][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(vt.at(j, blk, e), s[rt][0][j], acc[rt][db], 0, 0, 0);
+                    for (int j = 0; j < NJ; ++j)
+                        acc[rt][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(vt.at(j, blk, e), s[rt][j / 4][j % 4], acc[rt][db], 0, 0, 0);
             }
         }
         if (i + 1 < n_tiles) load_v(i + 1);
     }
 
-    // ---- join the waves ----
+    // ---- join the waves: out = sum_w O_w 2^(m_w - M) / sum_w l_w 2^(m_w - M) ----
+    // Four dims that lie side by side are one item; a lane has DB of them a row tile.  The items go
+    // through LDS in the lanes' own order, so that neither side meets a bank conflict.
+    auto put = [&](int rt) {
+        f32x4_t* to = s_acc + wave * DB * 64 + lane;
+#pragma unroll
+        for (int it = 0; it < DB; ++it) {
+            if (it < G::NBLK * G::E) {
+                constexpr int Q4 = G::E / 4;
+                const int db = it / G::E * G::E + it % Q4 * 4, r = it % G::E / Q4;
+                to[it * 64] = f32x4_t{acc[rt][db][r], acc[rt][db + 1][r], acc[rt][db + 2][r], acc[rt][db + 3][r]};
+            } else {
+                to[it * 64] = acc[rt][it];
+            }
+        }
+    };
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         float sum = l[rt];
@@ -500,40 +593,59 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT, W)) ffa_tr
             s_ml[wave][rt * 16 + c][1] = sum;
         }
     }
+    put(0);
     __syncthreads();
-    const bool whole = P.n_splits == 1;
-    const uint64_t bad = ((uint64_t)s_bad[1] << 32) | s_bad[0];
+    const bool whole = n_splits == 1, weights = P.ws_scores != nullptr;
+    if (tid < RT * 16) {
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) M = fmaxf(M, s_ml[w][tid][0]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float mw = s_ml[w][tid][0];
+            const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
+            L += f * s_ml[w][tid][1];
+            s_ml[w][tid][0] = f;
+        }
+        s_row[tid][0] = M;
+        s_row[tid][1] = L;
+        const int row = row0 + tid;
+        if ((!whole || weights) && row < P.rows) {
+            float* to = P.ws_ml + (((size_t)pair * n_splits + split) * P.rows + row) * 2;
+            to[0] = M;
+            to[1] = L;
+        }
+    }
+    uint64_t bad = 0;
+    if (last) {
+#pragma unroll
+        for (int d = 0; d < 64 / TK; ++d)
+            if (d * TK < count) bad |= s_bad[d] << (d * TK);
+    }
+    __syncthreads();
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const int mine = rt * 16 + c;
-        float top = s_ml[0][mine][0];
-#pragma unroll
-        for (int w = 1; w < W; ++w) top = fmaxf(top, s_ml[w][mine][0]);
-        const float f = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - top);
-        if (rt > 0) __syncthreads();
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                s_acc[wave * 16 * RS + c * RS + tile_dim<T, DH>(db, g * 4 + r)] = m[rt] == -INFINITY ? 0.f : acc[rt][db][r] * f;
-        __syncthreads();
-        // 16 rows x DH outputs, four dims a thread.
-        for (int i = tid; i < 16 * DH / 4; i += W * 64) {
-            const int r = i / (DH / 4), d = (i % (DH / 4)) * 4;
+        if (rt > 0) {
+            __syncthreads();
+            put(rt);
+            __syncthreads();
+        }
+        for (int i = tid; i < DB * 64; i += W * 64) {
+            const int it = i / 64, r = i % 16, gg = i / 16 % 4;
             const int row = row0 + rt * 16 + r;
             if (row >= P.rows) continue;
-            const int token = row / P.G;
-            float M = s_ml[0][rt * 16 + r][0];
-#pragma unroll
-            for (int w = 1; w < W; ++w) M = fmaxf(M, s_ml[w][rt * 16 + r][0]);
-            float L = 0.f;
+            constexpr int Q4 = G::E / 4;
+            const int d = it < G::NBLK * G::E ? it / G::E * 16 * G::E + (gg * 4 + it % G::E / Q4) * G::E + it % Q4 * 4
+                                              : G::NBLK * 16 * G::E + gg * 4;
             f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                const float mw = s_ml[w][rt * 16 + r][0];
-                if (mw != -INFINITY) L += s_ml[w][rt * 16 + r][1] * __builtin_amdgcn_exp2f(mw - M);
-                o += *reinterpret_cast<const f32x4_t*>(&s_acc[w * 16 * RS + r * RS + d]);
+                // A wave that counts nothing adds nothing, also where its sum is infinite.
+                const float f = s_ml[w][rt * 16 + r][0];
+                const f32x4_t x = s_acc[w * DB * 64 + i] * f;
+                o += f != 0.f ? x : f32x4_t{0.f, 0.f, 0.f, 0.f};
             }
+            const int token = quotient(row, P.G, P.G_magic);
             if (bad != 0) {
                 for (uint64_t todo = bad & s_seen[token]; todo != 0; todo &= todo - 1) {
                     const int node = __ffsll((unsigned long long)todo) - 1;
@@ -545,36 +657,25 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT, W)) ffa_tr
                     }
                 }
             }
-            const size_t slot = ((size_t)pair * P.n_splits + split) * P.rows + row;
-            if (P.ws_scores != nullptr && P.score_lds != 0 && d == 0) {
-                s_row[r][0] = -M;
-                s_row[r][1] = 1.f / L;
-            }
-            if ((!whole || P.ws_scores != nullptr) && d == 0) {
-                P.ws_ml[slot * 2] = M;
-                P.ws_ml[slot * 2 + 1] = L;
-            }
             if (!whole) {
-                *reinterpret_cast<f32x4_t*>(P.ws_acc + slot * DH + d) = o;
+                *reinterpret_cast<f32x4_t*>(P.ws_acc + (((size_t)pair * n_splits + split) * P.rows + row) * DH + d) = o;
             } else if (token < count) {
-                const int gh = row % P.G;
-                T* to = static_cast<T*>(P.out) + b * P.out_stride[0] + (long long)(h * P.G + gh) * P.out_stride[1] + token * P.out_stride[2];
-                store_out4(to + d, o / L);
+                T* to = static_cast<T*>(P.out) + b * P.out_stride[0] + (long long)(h * P.G + row - token * P.G) * P.out_stride[1] + token * P.out_stride[2];
+                store_out4(to + d, o / s_row[rt * 16 + r][1]);
             }
         }
     }
 
     // ---- weight-summing step with scores in LDS (one row tile): the weights if this piece is all there
     // is, else the scores go to the workspace, where the pieces' kernel finds them ----
-    if (P.ws_scores != nullptr && P.score_lds != 0) {
-        __syncthreads();
-        const int from = max(first, piece0), to = min(length, piece0 + P.tiles_per_split * TK);
+    if (weights && P.score_lds != 0) {
+        const int from = max(first, piece0), to = min(length, piece0 + tiles_per_split * TK);
         if (whole) {
-            float* kw = P.key_weights + (size_t)pair * P.Lmax;
+            float* kw = P.key_weights + (size_t)pair * Lmax;
             for (int j = from + tid; j <= to; j += W * 64) {
                 float w = 0.f;
                 for (int r = 0; r < P.rows; ++r)
-                    w += __builtin_amdgcn_exp2f(s_scores[r * P.score_lds + (j == length ? P.score_lds - 32 : j - piece0)] + s_row[r][0]) * s_row[r][1];
+                    w += __builtin_amdgcn_exp2f(s_scores[r * P.score_lds + (j == length ? P.score_lds - 64 : j - piece0)] - s_row[r][0]) / s_row[r][1];
                 if (j == length) kw[j] = w;
                 else kw[j] += w;
             }
@@ -582,21 +683,8 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT, W)) ffa_tr
             for (int r = 0; r < P.rows; ++r) {
                 float* ws = P.ws_scores + ((size_t)pair * P.rows + r) * P.score_stride;
                 for (int j = from + tid; j < to; j += W * 64) ws[j] = s_scores[r * P.score_lds + j - piece0];
-                if (last && tid == 0) ws[P.score_stride - 32] = s_scores[r * P.score_lds + P.score_lds - 32];
+                if (last && tid == 0) ws[P.score_stride - 64] = s_scores[r * P.score_lds + P.score_lds - 64];
             }
-        }
-    }
-
-    // ---- append the new tokens: no one reads cache slots from `length` on ----
-    if (last && rb == 0) {
-        char* kw = const_cast<char*>(kc);
-        char* vw = const_cast<char*>(vc);
-        for (int i = tid; i < count * NCH; i += W * 64) {
-            const int node = i / NCH, ch = i % NCH, slot = length + node;
-            const uint4 x = *reinterpret_cast<const uint4*>(kn + node * kn_row + ch * 16);
-            const uint4 y = *reinterpret_cast<const uint4*>(vn + node * vn_row + ch * 16);
-            st16(kw + ((size_t)ch * P.Lmax + slot) * 16, x);
-            st16(vw + slot * cache_row + ch * 16, y);
         }
     }
 }
@@ -671,7 +759,7 @@ __global__ void __launch_bounds__(256) ffa_tree_finish_kernel(const TreeParams P
     for (int row = 0; row < P.rows; ++row) {
         const RowTotal t = row_total(P, (size_t)pair * P.n_splits * P.rows + row);
         const float* x = P.ws_scores + ((size_t)pair * P.rows + row) * P.score_stride;
-        w += __builtin_amdgcn_exp2f(x[j == length ? P.score_stride - 32 : j] - t.M) / t.L;
+        w += __builtin_amdgcn_exp2f(x[j == length ? P.score_stride - 64 : j] - t.M) / t.L;
     }
     float* to = P.key_weights + (size_t)pair * P.Lmax + j;
     if (j == length) *to = w;
@@ -680,25 +768,27 @@ __global__ void __launch_bounds__(256) ffa_tree_finish_kernel(const TreeParams P
 
 // ---------------------------------------------------------------------------------------
 template <typename T, int DH, int RT, int W> int launch_tree_kernel(const TreeParams& P, hipStream_t st) {
-    const int pieces = P.B * P.H * P.n_splits;
-    const dim3 grid((unsigned)((pieces + 7) / 8 * 8 * P.row_blocks));
+    const dim3 grid(8u * (unsigned)P.row_blocks, (unsigned)((P.B * P.H * P.n_splits + 7) / 8));
     const size_t lds = (size_t)(tree_merge_floats<DH, W>() + P.rows * P.score_lds) * sizeof(float);
-    hipLaunchKernelGGL((ffa_tree_kernel<T, DH, RT, W>), grid, dim3(W * 64), lds, st, P);
+    hipLaunchKernelGGL((ffa_tree_kernel<T, DH, RT, W>), grid, dim3(W * 64), lds, st, TREE_HOT_OF(P), P);
     return hipGetLastError() == hipSuccess ? FFA_OK : FFA_ERR_LAUNCH;
 }
 
 template <typename T, int DH> int launch_tree_dh(const TreeParams& P, const TreePlan& plan, hipStream_t st) {
     int rc = FFA_ERR_PLAN;
     if (plan.waves > 4) {
-        if constexpr (DH != 256) {
-            constexpr int W = tree_wide_waves(DH, 1);
-            if (plan.row_tiles == 1 && plan.waves == W) rc = launch_tree_kernel<T, DH, 1, W>(P, st);
-        }
-        if constexpr (tree_wide_waves(DH, 2) != 0)
-            if (plan.row_tiles == 2 && plan.waves == tree_wide_waves(DH, 2)) rc = launch_tree_kernel<T, DH, 2, tree_wide_waves(DH, 2)>(P, st);
+        if constexpr (tree_wide(DH, 1))
+            if (plan.row_tiles == 1) rc = launch_tree_kernel<T, DH, 1, 8>(P, st);
+        if constexpr (tree_wide(DH, 2))
+            if (plan.row_tiles == 2) rc = launch_tree_kernel<T, DH, 2, 8>(P, st);
+        if constexpr (tree_wide(DH, 3))
+            if (plan.row_tiles == 3) rc = launch_tree_kernel<T, DH, 3, 8>(P, st);
+        if constexpr (tree_wide(DH, 4))
+            if (plan.row_tiles == 4) rc = launch_tree_kernel<T, DH, 4, 8>(P, st);
     } else {
         if (plan.row_tiles == 1) rc = launch_tree_kernel<T, DH, 1, 4>(P, st);
-        if (plan.row_tiles == 2) rc = launch_tree_kernel<T, DH, 2, 4>(P, st);
+        if constexpr (tree_row_tiles(DH) > 1)
+            if (plan.row_tiles == 2) rc = launch_tree_kernel<T, DH, 2, 4>(P, st);
         if constexpr (tree_row_tiles(DH) > 2)
             if (plan.row_tiles == 3) rc = launch_tree_kernel<T, DH, 3, 4>(P, st);
         if constexpr (tree_row_tiles(DH) > 3)

@@ -111,13 +111,14 @@ torch::Tensor int_input(const OptTensor& x, const torch::Tensor& like, at::IntAr
 const int* int_ptr(const torch::Tensor& x) { return x.defined() ? x.data_ptr<int>() : nullptr; }
 
 // [B, heads, n, Dh] in any order of its first three dimensions; copied only if a row is not
-// contiguous or not made of aligned 16-byte pieces.
+// contiguous, not made of aligned 16-byte pieces, or too far from the next.
 torch::Tensor group_input(const torch::Tensor& x, const torch::Tensor& like, const char* name) {
     TORCH_CHECK(x.device() == like.device() && x.scalar_type() == like.scalar_type(), "ff_attention: ", name,
                 " must have the caches' dtype and device");
     const int64_t unit = 16 / x.element_size();
     bool fits = x.stride(3) == 1 && (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) == 0;
     for (int i = 0; i < 3; ++i) fits = fits && x.stride(i) % unit == 0;
+    fits = fits && x.stride(2) * x.element_size() < (1 << 26);
     return fits ? x : x.clone(at::MemoryFormat::Contiguous);
 }
 
