@@ -85,6 +85,7 @@ struct EvictParams {
     const int *first_keys, *lengths;
     int* kept;  // [n_caches, B, H, keep]
     int n_caches, B, H, src_len, dst_len, t, keep, recent;
+    int segment_batches;  // batches of a wave's walk through the kept slots
 };
 int launch_evict(const EvictParams& P, int head_dim, int elem_bytes, void* stream);
 

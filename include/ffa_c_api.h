@@ -356,7 +356,8 @@ int ffa_attention_tree(int precision, int batch_size, int head_num, int head_dim
  * sample's length, K and V, in n_caches caches of one shape (one a layer) in one call:
  *   for j < accepted[b]:  slot length + j  <-  the old slot length + path[b, j].
  * path [B, path_len] holds node numbers as attention_tree counts them, root first (so each is
- * larger than the one before); accepted [B] is clamped to [0, path_len], and a slot to the cache.
+ * larger than the one before); accepted [B] is clamped to [0, path_len], a node to
+ * [0, FFA_MAX_TREE_TOKENS - 1] and to the cache.
  * All old slots of a sample are read before any is written, so that every path is a gather.
  * path_len 1 .. FFA_MAX_TREE_TOKENS; k_caches and v_caches are HOST arrays of device pointers.
  */
