@@ -28,6 +28,14 @@ Written against the installed transformers (5.x) instead of a patched copy of it
   (`attention_ex(..., cache_indir, beam_width)`: the FasterTransformer feature of
   attention.cu:1024-1033 that the reference switches off).  Keys and values never move.
 
+* passes of several tokens after the prompt (a prompt in chunks, assisted and prompt-lookup
+  decoding), which the reference's models cannot run, go to `attention_tree` as chains of up to 64
+  tokens; `crop` takes rejected tokens back.
+* a cache of bounded size (`FFACache(..., keep=n, recent=m)`): every step goes to
+  `attention_weights`, which sums the attention each key receives, starting from the prompt's own;
+  whenever evict_every tokens have come on top of `keep`, `evict` keeps the last `recent` tokens
+  and the heaviest of the others, per head.
+
     from fastforwardattention_amd import hf
     hf.enable(model)
     out = model.generate(ids, attention_mask=mask, max_new_tokens=n,
@@ -56,15 +64,24 @@ def _default_engine():
 
 
 class FFALayer(CacheLayerMixin):
-    """One decoder layer's cache: a `FastForwardAttn` built at the prompt pass, the number of
-    keys it holds, and the left-padding offsets of the batch."""
+    """One decoder layer's cache: a `FastForwardAttn` built at the prompt pass (or the bounded caches
+    filled from it), the number of keys it holds, and the left-padding offsets of the batch."""
 
     is_sliding = False
     is_compileable = False
 
     def __init__(self, max_new_tokens: int, prob_thresh: float = 0.0,
-                 use_default_kernel_launch: bool = False, engine=None, num_beams: int = 1):
+                 use_default_kernel_launch: bool = False, engine=None, num_beams: int = 1,
+                 keep: int | None = None, recent: int | None = None, evict_every: int = 64):
         super().__init__()
+        if keep is not None:
+            recent = keep // 2 if recent is None else recent
+            if keep < 1 or not 0 <= recent <= keep or evict_every < 1:
+                raise ValueError("eviction wants keep >= 1, 0 <= recent <= keep and evict_every >= 1")
+            if num_beams != 1 or prob_thresh != 0.0:
+                raise ValueError("eviction goes with neither beam search nor a pruning threshold")
+        self.keep, self.recent, self.evict_every = keep, recent, int(evict_every)
+        self.bounded = None         # (k_cache, v_cache, key_weights) of keep + evict_every slots
         if max_new_tokens < 1:
             raise ValueError("max_new_tokens must be >= 1")
         if num_beams < 1:
@@ -76,7 +93,8 @@ class FFALayer(CacheLayerMixin):
         self.use_default_kernel_launch = bool(use_default_kernel_launch)
         self._engine_cls = engine
         self.engine = None
-        self.t = 0                  # keys cached so far = slot of the next token
+        self.t = 0                  # keys cached = slot of the next token
+        self.seen = 0               # tokens so far: more than t once some were evicted
         self.max_len = 0
         self.first_key = None       # int32 [B]: first real key of each left-padded sample
         self._hooked = False        # the attention hook has seen this layer's prompt pass
@@ -88,30 +106,42 @@ class FFALayer(CacheLayerMixin):
         self.is_initialized = True
 
     def update(self, key_states, value_states, *args, **kwargs):
-        if key_states.shape[-2] != 1 or self.engine is None:
+        if self.engine is None:
             return self._prompt_pass(key_states, value_states)
+        n = key_states.shape[-2]
+        if n > 1:
+            self._check_group_pass()
         if not self._hooked:
             raise RuntimeError("FFACache: the model's attention does not go through the 'ffa' hook; "
                                "call fastforwardattention_amd.hf.enable(model) first")
         if self._pending:
             raise RuntimeError("FFACache: the previous decode token of this layer was never attended")
-        if self.t >= self.max_len:
-            raise RuntimeError(f"FFACache: cache full ({self.max_len} slots = prompt + max_new_tokens)")
+        self._check_room(n)
         self._pending = True
         setattr(key_states, _TAG, self)
         return key_states, value_states
 
+    def _check_room(self, n):
+        if self.seen + n > self.max_len:
+            raise RuntimeError(f"FFACache: cache full ({self.max_len} slots = prompt + max_new_tokens)")
+
+    def _check_group_pass(self):
+        if self.beam_table is not None or self.bounded is not None or not hasattr(self.engine, "attention_tree"):
+            raise NotImplementedError("FFACache: passes of several tokens after the prompt need an engine with attention_tree "
+                                      "and go with neither beam search nor eviction")
+
     def get_seq_length(self) -> int:
-        return self.t
+        return self.seen
 
     def get_mask_sizes(self, query_length: int):
-        return self.t + query_length, 0
+        return self.seen + query_length, 0
 
     def get_max_length(self) -> int:
         return -1
 
     def reset(self):
         self.engine, self.t, self.max_len, self.first_key, self.beam_table = None, 0, 0, None, None
+        self.seen, self.bounded = 0, None
         self._hooked = self._pending = False
 
     def reorder_cache(self, beam_idx):
@@ -132,25 +162,36 @@ class FFALayer(CacheLayerMixin):
         table[:, self.t - 1] = (beam_idx % self.num_beams).to(torch.int32)
         self.beam_table = table
 
-    def _unsupported(self, *a, **k):
-        raise NotImplementedError("FFACache holds the reference's fixed-layout caches: no cropping or batch "
-                                  "reshaping")
+    def crop(self, max_length: int):
+        """Forgets the tokens from `max_length` on (zero or negative: that many of the last, as transformers'
+        own caches take it): their slots are written again by the tokens that come instead."""
+        if self.engine is None or self.beam_table is not None or self.bounded is not None:
+            raise NotImplementedError("FFACache: cropping needs a prompt and goes with neither beam search nor eviction")
+        max_length = int(max_length)
+        if max_length <= 0:
+            max_length = max(0, self.seen + max_length)
+        self.t = self.seen = min(self.seen, max_length)
+        self._pending = False
 
-    crop = batch_repeat_interleave = batch_select_indices = offload = prefetch = _unsupported
+    def _unsupported(self, *a, **k):
+        raise NotImplementedError("FFACache holds the reference's fixed-layout caches: no batch reshaping")
+
+    batch_repeat_interleave = batch_select_indices = offload = prefetch = _unsupported
 
     # -- the two passes -------------------------------------------------------------------
     def _prompt_pass(self, key_states, value_states):
-        if self.engine is not None:
-            raise NotImplementedError("FFACache: a second multi-token pass (chunked prefill, assisted decoding) "
-                                      "is not supported; the reference builds its caches from one prompt pass")
         if not self.is_initialized:
             self.lazy_initialization(key_states, value_states)
         cls = self._engine_cls or _default_engine()
         prompt_len = key_states.shape[-2]
         self.max_len = prompt_len + self.max_new_tokens
+        if self.keep is not None and not (hasattr(cls, "attention_weights") and hasattr(cls, "evict")):
+            raise NotImplementedError("FFACache: this engine has no attention_weights and evict, which keep= needs")
+        # A bounded cache is filled from the prompt's once the prompt's attention is known.
+        slots = prompt_len if self.keep is not None else self.max_len
         self.engine = cls(key_states.contiguous(), value_states.to(key_states.dtype).contiguous(),
-                          self.max_len, self.use_default_kernel_launch)
-        self.t = prompt_len
+                          slots, self.use_default_kernel_launch)
+        self.t = self.seen = prompt_len
         if self.num_beams > 1:
             B = key_states.shape[0]
             if B % self.num_beams:
@@ -174,12 +215,63 @@ class FFALayer(CacheLayerMixin):
             row = row.to(torch.int8)
         self.first_key = torch.max(row, dim=-1).indices.reshape(-1).to(torch.int32).contiguous()
 
+    def note_prompt_weights(self, weights):
+        """The prompt pass's attention weights [B,H,Lq,Lk], for a bounded cache: what each key received
+        from real queries.  Moves the prompt into the bounded caches."""
+        if self.keep is None:
+            return
+        w = weights.float()
+        if self.first_key is not None:      # the rows of padding say nothing
+            real = torch.arange(w.shape[2], device=w.device)[None] >= self.first_key[:, None]
+            w = torch.where(real[:, None, :, None], w, 0.0)
+        w = w.sum(2).contiguous()
+        k, v = self.engine.get_cache()
+        cap = self.keep + self.evict_every
+        self.bounded = (k.new_empty((*k.shape[:3], cap, k.shape[4])), v.new_empty((*v.shape[:2], cap, v.shape[3])),
+                        w.new_zeros((*w.shape[:2], cap)))
+        self.engine = type(self.engine)     # its caches are not needed any more
+        self._evict([(k, v)], [w], [self.bounded])
+
+    def _evict(self, caches, weights, into):
+        self.engine.evict(caches, weights, self.t, self.keep, self.recent, first_keys=self.first_key, into=into)
+        gone = max(0, self.t - self.keep)
+        if self.first_key is not None:      # padding goes first
+            self.first_key = (self.first_key - gone).clamp_(min=0)
+        self.t -= gone
+
+    def attend_group(self, query, key, value, scale: float):
+        """A pass of n tokens after the prompt: [B,H,n,Dh] q/k/v -> [B,H,n,Dh]; appends them from slot t on."""
+        if not self._pending:
+            raise RuntimeError("FFACache: attend_group() without pending tokens")
+        dt, n = self.dtype, key.shape[-2]
+        q, k, v = query.to(dt), key.to(dt), value.to(dt)
+        k_cache, v_cache = self.engine.get_cache()
+        outs = []
+        for i in range(0, n, 64):
+            part = slice(i, min(n, i + 64))
+            outs.append(self.engine.attention_tree(q[:, :, part], k[:, :, part], v[:, :, part], k_cache, v_cache,
+                                                   float(scale), self.t + i, first_keys=self.first_key))
+        self.t += n
+        self.seen += n
+        self._pending = False
+        return outs[0] if len(outs) == 1 else torch.cat(outs, dim=2)
+
     def attend(self, query, key, value, scale: float):
         """One decode step: [B,H,1,Dh] q/k/v -> [B,H,Dh]; appends k, v at slot t."""
         if not self._pending:
             raise RuntimeError("FFACache: attend() without a pending decode token")
         dt = self.dtype
         q, k, v = query.to(dt), key.to(dt), value.to(dt)
+        if self.bounded is not None:
+            k_cache, v_cache, w = self.bounded
+            if self.t == w.shape[2]:
+                self._evict([(k_cache, v_cache)], [w], None)
+            out = self.engine.attention_weights(q, k, v, k_cache, v_cache, float(scale), self.t, w,
+                                                first_keys=self.first_key)
+            self.t += 1
+            self.seen += 1
+            self._pending = False
+            return out
         k_cache, v_cache = self.engine.get_cache()
         if self.beam_table is not None:
             out = self.engine.attention_ex(q, k, v, k_cache, v_cache, float(scale), self.t, self.first_key,
@@ -191,6 +283,7 @@ class FFALayer(CacheLayerMixin):
             out = self.engine.attention(q, k, v, k_cache, v_cache, float(scale), self.t, self.first_key,
                                         self.prob_thresh)
         self.t += 1
+        self.seen += 1
         self._pending = False
         return out
 
@@ -200,14 +293,14 @@ class FFALayer(CacheLayerMixin):
         transformers passes as position_ids for a left-padded batch) and appends."""
         if not self._hooked:
             raise RuntimeError("FFACache: the prompt pass did not go through the 'ffa' hook")
-        if self.t >= self.max_len:
-            raise RuntimeError(f"FFACache: cache full ({self.max_len} slots = prompt + max_new_tokens)")
+        self._check_room(1)
         dt = self.dtype
         k_cache, v_cache = self.engine.get_cache()
         beams = {} if self.beam_table is None else dict(cache_indir=self.beam_table, beam_width=self.num_beams)
         out = self.engine.attention_ex(query.to(dt), key.to(dt), value.to(dt), k_cache, v_cache, float(scale), self.t,
                                        self.first_key, self.prob_thresh, int(rotary_dim), None, None, None, **beams)
         self.t += 1
+        self.seen += 1
         return out
 
 
@@ -216,12 +309,16 @@ class FFACache(Cache):
     `FastForwardAttn` (cache layouts [B,H,Dh/x,Lmax,x] / [B,H,Lmax,Dh], Lmax = prompt +
     max_new_tokens).  `engine` replaces the `FastForwardAttn` class (same constructor and
     methods); tests use it to run the bookkeeping without a GPU.  num_beams: generate's num_beams
-    when beam search is used (samples are grouped num_beams at a time, as generate lays them out)."""
+    when beam search is used (samples are grouped num_beams at a time, as generate lays them out).
+    keep: bound the cache: keep + evict_every slots a head; when they are full, `keep` stay: the last
+    `recent` tokens (default keep // 2) and of the others those that received the most attention, by
+    head.  Memory and step time then do not grow with the sequence."""
 
     def __init__(self, max_new_tokens: int, prob_thresh: float = 0.0,
-                 use_default_kernel_launch: bool = False, engine=None, num_beams: int = 1):
+                 use_default_kernel_launch: bool = False, engine=None, num_beams: int = 1,
+                 keep: int | None = None, recent: int | None = None, evict_every: int = 64):
         super().__init__(layer_class_to_replicate=functools.partial(
-            FFALayer, max_new_tokens, prob_thresh, use_default_kernel_launch, engine, num_beams))
+            FFALayer, max_new_tokens, prob_thresh, use_default_kernel_launch, engine, num_beams, keep, recent, evict_every))
 
     @classmethod
     def from_env(cls, engine=None):
@@ -237,12 +334,12 @@ def enabled_by_env() -> bool:
 
 # -- attention hooks --------------------------------------------------------------------------
 def _plain_attention(query, key, value, attention_mask, scaling):
-    """Ordinary masked softmax attention for the prompt pass; [B,H,Lq,Dh] in and out."""
+    """Ordinary masked softmax attention for the prompt pass: [B,H,Lq,Dh] and the weights [B,H,Lq,Lk]."""
     w = torch.matmul(query, key.transpose(-1, -2)) * scaling
     if attention_mask is not None:
         w = w + attention_mask if attention_mask.dtype != torch.bool else w.masked_fill(~attention_mask, float("-inf"))
     w = torch.softmax(w, dim=-1, dtype=torch.float32).to(value.dtype)
-    return torch.matmul(w, value)
+    return torch.matmul(w, value), w
 
 
 def ffa_attention_forward(module, query, key, value, attention_mask, scaling=None, dropout=0.0, **kwargs):
@@ -252,10 +349,14 @@ def ffa_attention_forward(module, query, key, value, attention_mask, scaling=Non
         scaling = query.shape[-1] ** -0.5
     layer = getattr(key, _TAG, None)
     if layer is not None and layer._pending:
+        if query.shape[-2] > 1:
+            return layer.attend_group(query, key, value, scaling).transpose(1, 2).contiguous(), None
         return layer.attend(query, key, value, scaling).unsqueeze(1), None
     if layer is not None:
         layer.note_prompt_mask(attention_mask)
-    out = _plain_attention(query, key, value, attention_mask, scaling)
+    out, weights = _plain_attention(query, key, value, attention_mask, scaling)
+    if layer is not None:
+        layer.note_prompt_weights(weights)
     return out.transpose(1, 2).contiguous(), None
 
 
@@ -263,10 +364,15 @@ def _gptj_attn(self, query, key, value, attention_mask=None, *rest):
     """Replacement for GPTJAttention._attn (modeling_gptj.py:252-281): ([B,H,Lq,Dh], weights)."""
     layer = getattr(key, _TAG, None)
     if layer is not None and layer._pending:
+        if query.shape[-2] > 1:
+            return layer.attend_group(query, key, value, 1.0 / self.scale_attn), None
         return layer.attend(query, key, value, 1.0 / self.scale_attn).unsqueeze(2), None
     if layer is not None:
         layer.note_prompt_mask(attention_mask)
-    return self._ffa_original_attn(query, key, value, attention_mask, *rest)
+    out, weights = self._ffa_original_attn(query, key, value, attention_mask, *rest)
+    if layer is not None:
+        layer.note_prompt_weights(weights)
+    return out, weights
 
 
 def _gptj_forward(self, hidden_states, layer_past=None, attention_mask=None, position_ids=None, use_cache=False,
@@ -277,8 +383,9 @@ def _gptj_forward(self, hidden_states, layer_past=None, attention_mask=None, pos
     layer = None
     if isinstance(layer_past, FFACache) and self.layer_idx is not None and len(layer_past.layers) > self.layer_idx:
         layer = layer_past.layers[self.layer_idx]
-    if (layer is None or layer.engine is None or hidden_states.shape[1] != 1 or output_attentions
-            or not hasattr(layer.engine, "attention_ex")):
+    # The engine rotates by the slot's distance from the first key: not the token's position after an eviction.
+    if (layer is None or layer.engine is None or layer.bounded is not None or hidden_states.shape[1] != 1
+            or output_attentions or not hasattr(layer.engine, "attention_ex")):
         return self._ffa_original_forward(hidden_states, layer_past, attention_mask, position_ids, use_cache,
                                           output_attentions, **kwargs)
     B, H, Dh = hidden_states.shape[0], self.num_attention_heads, self.head_dim
