@@ -63,7 +63,7 @@ class BeamIndirection(C.Structure):
 class TreeTokens(C.Structure):
     """struct ffa_tree_tokens."""
     _fields_ = [("tokens", C.c_int32), ("q_head_num", C.c_int32), ("parents", C.c_void_p), ("first_keys", C.c_void_p),
-                ("lengths", C.c_void_p), ("counts", C.c_void_p), ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3),
+                ("lengths", C.c_void_p), ("counts", C.c_void_p), ("zero_rest", C.c_int32), ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3),
                 ("v_stride", C.c_int64 * 3), ("out_stride", C.c_int64 * 3)]
 
 

@@ -64,7 +64,12 @@ struct TreeShape {
 TreeShape tree_shape(int precision, int pairs, int rows, int head_dim, int t, int cus) {
     TreeShape s;
     const int row_tiles = ceil_div(rows, 16);
-    s.row_blocks = ceil_div(row_tiles, tree_row_tiles(head_dim));
+    // On few keys a workgroup's fixed cost counts, which grows with its rows, more than reading the keys
+    // again (256 pairs, 64 rows, two and four row tiles, 0, 512, 2000 keys: Dh 128 12.4 and 16.6, 23.4 and 27.6,
+    // 84 and 71 us; Dh 64 9.6 and 10.7, 16.5 and 17.6, 38.3 and 37.6 us), and one row tile is best where all
+    // workgroups run at once (2 pairs, 472 rows, 267 keys, Dh 256: one 14, two 21 us).
+    const int few = pairs * row_tiles <= cus ? 1 : 2;
+    s.row_blocks = ceil_div(row_tiles, t <= 768 ? few : tree_row_tiles(head_dim));
     s.row_tiles = ceil_div(row_tiles, s.row_blocks);
     s.tile_keys = 16 * tree_tile_units(elem_bytes(precision), head_dim, s.row_tiles);
     const int tiles = ceil_div(t, s.tile_keys), groups = pairs * s.row_blocks;
@@ -188,6 +193,7 @@ int ffa_attention_tree(int precision, int batch_size, int head_num, int head_dim
     P.k_cache = k_cache; P.v_cache = v_cache; P.out = out;
     P.parents = tokens->parents; P.first_keys = tokens->first_keys;
     P.lengths = tokens->lengths; P.counts = tokens->counts;
+    P.zero_rest = tokens->zero_rest;
     for (int i = 0; i < 3; ++i) {
         P.q_stride[i] = tokens->q_stride[i]; P.k_stride[i] = tokens->k_stride[i];
         P.v_stride[i] = tokens->v_stride[i]; P.out_stride[i] = tokens->out_stride[i];

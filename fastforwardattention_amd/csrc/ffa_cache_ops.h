@@ -20,8 +20,8 @@ constexpr int tree_tile_units(int elem_bytes, int head_dim, int row_tiles) {
     return (elem_bytes == 2 ? 2 : 1) * (row_tiles == 1 && head_dim <= 80 ? 2 : 1);
 }
 
-// Most 16-row matrix tiles a wave holds without spilling registers.
-constexpr int tree_row_tiles(int head_dim) { return head_dim == 256 ? 1 : 4; }
+// Most 16-row matrix tiles a wave's registers hold.
+constexpr int tree_row_tiles(int head_dim) { return head_dim == 256 ? 2 : 4; }
 
 // Whether two waves a SIMD fit the registers.
 constexpr bool tree_two_waves(int head_dim, int row_tiles) { return head_dim <= 128 && head_dim * row_tiles <= 256; }
@@ -51,6 +51,7 @@ struct TreeParams {
     int score_lds;       // as in the plan
     int B, H, G, tokens, rows, Lmax, t;
     float scale_log2e;  // |softmax_scale| * log2(e), never zero
+    int zero_rest;      // rows past a sample's count are set to zero
     int q_sign;         // sign of softmax_scale: Q enters with it
     int n_splits, tiles_per_split, row_blocks;
     unsigned splits_magic, H_magic, G_magic;  // tree_magic() of n_splits, H and G

@@ -243,8 +243,16 @@ __device__ __forceinline__ uint64_t ancestor_mask(const int* parents, int tokens
 // other's matrix products; what holds more than 256 registers of results and operands runs alone.
 constexpr int tree_waves_per_simd(int dh, int rt) { return tree_two_waves(dh, rt) ? 2 : 1; }
 
-// Floats of LDS in front of the scores: the waves' results of one row tile.
+// Q fragments of all row tiles, one register quadruple each: from 8 of them on they are read from LDS at
+// every tile (128 cycles of it a wave at 16) and leave their registers to results and loads.  At 256 pairs
+// of 8000 keys, in registers and in LDS: Dh 128, 64 rows 251 and 191 us (registers spilled), 32 rows 164
+// and 155 us; Dh 64, 64 rows alike, at 1000 keys 25.3 and 23.6 us.
+template <typename T, int DH, int RT> constexpr bool tree_q_in_lds() { return RT * TreeGeo<T, DH, RT>::KK >= 8; }
+// Floats of LDS in front of the scores: the waves' results of one row tile, and Q.
 template <int DH, int W> constexpr int tree_merge_floats() { return W * 16 * DH; }
+template <typename T, int DH, int RT> constexpr int tree_q_floats() {
+    return tree_q_in_lds<T, DH, RT>() ? RT * TreeGeo<T, DH, RT>::KK * 64 * 4 : 0;
+}
 
 // Arguments that the first loads need, ahead of the struct: they arrive in registers with the wave.
 #define TREE_HOT_DECL const char *k_cache, const char *v_cache, int Lmax, int t, int n_splits, unsigned splits_magic, \
@@ -258,10 +266,12 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT)) ffa_tree_
     using G = TreeGeo<T, DH, RT>;
     constexpr int NU = G::NU, TK = G::TK, KK = G::KK, NCH = G::NCH, DB = G::DB, NJ = 4 * NU;
     constexpr unsigned ROW = DH * sizeof(T);  // bytes of a cache row
+    constexpr bool QLDS = tree_q_in_lds<T, DH, RT>();
     constexpr bool SHORT = RT == 1;           // few new tokens are likely: skip 16 keys that hold none
     extern __shared__ float4 s_dynamic[];
     f32x4_t* const s_acc = reinterpret_cast<f32x4_t*>(s_dynamic);                               // [W][DB][64]
-    float* const s_scores = reinterpret_cast<float*>(s_dynamic) + tree_merge_floats<DH, W>();   // [rows][score_lds]
+    uint4* const s_q = reinterpret_cast<uint4*>(s_acc + W * DB * 64);                           // [RT][KK][64]
+    float* const s_scores = reinterpret_cast<float*>(s_dynamic) + tree_merge_floats<DH, W>() + tree_q_floats<T, DH, RT>();  // [rows][score_lds]
     __shared__ float s_ml[W][RT * 16][2];  // a wave's m and l of a row; then s_ml[..][0] = its factor
     __shared__ float s_row[RT * 16][2];    // M and L of a row
     __shared__ uint64_t s_seen[64];
@@ -369,25 +379,28 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT)) ffa_tree_
 
     // Q: chunk kk * 4 + g of row row0 + rt * 16 + c; rows and chunks that do not exist are zero.
     // The factor of the scores is positive: a negative softmax_scale turns Q's sign.
-    uint4 qf[RT][KK];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int row = row0 + rt * 16 + c;
+    auto load_q = [&](int rt, int kk) {
+        const int row = row0 + rt * 16 + c, ch = kk * 4 + g;
         const int token = quotient(row, P.G, P.G_magic), gh = row - token * P.G;
-        const char* qr = static_cast<const char*>(P.q) +
-                         (b * P.q_stride[0] + (long long)(h * P.G + gh) * P.q_stride[1] + token * P.q_stride[2]) * (long long)sizeof(T);
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-            const int ch = kk * 4 + g;
-            qf[rt][kk] = make_uint4(0, 0, 0, 0);
-            if (row < P.rows && ch < NCH && P.q_sign != 0) {
-                constexpr uint32_t sign = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
-                const uint32_t turn = P.q_sign < 0 ? sign : 0u;
-                uint4 x = *reinterpret_cast<const uint4*>(qr + ch * 16);
-                x.x ^= turn; x.y ^= turn; x.z ^= turn; x.w ^= turn;
-                qf[rt][kk] = x;
-            }
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (row < P.rows && ch < NCH && P.q_sign != 0) {
+            constexpr uint32_t sign = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+            const uint32_t turn = P.q_sign < 0 ? sign : 0u;
+            x = *reinterpret_cast<const uint4*>(static_cast<const char*>(P.q) + ch * 16 +
+                                                (b * P.q_stride[0] + (long long)(h * P.G + gh) * P.q_stride[1] + token * P.q_stride[2]) * (long long)sizeof(T));
+            x.x ^= turn; x.y ^= turn; x.z ^= turn; x.w ^= turn;
         }
+        return x;
+    };
+    uint4 qf[QLDS ? 1 : RT][QLDS ? 1 : KK];
+    if constexpr (QLDS) {
+        for (int i = wave; i < RT * KK; i += W) s_q[i * 64 + lane] = load_q(i / KK, i % KK);
+        __syncthreads();
+    } else {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) qf[rt][kk] = load_q(rt, kk);
     }
 
     f32x4_t acc[RT][DB];
@@ -424,6 +437,7 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT)) ffa_tree_
                 if (node < count) vt.store(j, vw + (size_t)(length + node) * ROW, c);
             }
         }
+        if constexpr (QLDS) asm volatile("" ::: "memory");  // Q stays in LDS: its registers are wanted
         f32x4_t s[RT][NU];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -431,7 +445,8 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT)) ffa_tree_
             for (int u = 0; u < NU; ++u) {
                 s[rt][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk) s[rt][u] = mma_qk(kf[u][kk], qf[rt][kk], s[rt][u], T{});
+                for (int kk = 0; kk < KK; ++kk)
+                    s[rt][u] = mma_qk(kf[u][kk], QLDS ? s_q[(rt * KK + kk) * 64 + lane] : qf[QLDS ? 0 : rt][QLDS ? 0 : kk], s[rt][u], T{});
             }
         if (i + 1 < n_tiles) load_k(i + 1);
         if (masked) {
@@ -659,9 +674,9 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT)) ffa_tree_
             }
             if (!whole) {
                 *reinterpret_cast<f32x4_t*>(P.ws_acc + (((size_t)pair * n_splits + split) * P.rows + row) * DH + d) = o;
-            } else if (token < count) {
+            } else if (token < count || P.zero_rest) {
                 T* to = static_cast<T*>(P.out) + b * P.out_stride[0] + (long long)(h * P.G + row - token * P.G) * P.out_stride[1] + token * P.out_stride[2];
-                store_out4(to + d, o / s_row[rt * 16 + r][1]);
+                store_out4(to + d, token < count ? o / s_row[rt * 16 + r][1] : f32x4_t{0.f, 0.f, 0.f, 0.f});
             }
         }
     }
@@ -712,7 +727,8 @@ __global__ void __launch_bounds__(256) ffa_tree_finish_kernel(const TreeParams P
         if (line >= (long long)P.B * P.H * P.rows) return;
         const int pair = (int)(line / P.rows), row = (int)(line % P.rows);
         const int b = pair / P.H, h = pair % P.H, token = row / P.G;
-        if (P.counts && token >= P.counts[b]) return;
+        const bool there = P.counts == nullptr || token < P.counts[b];
+        if (!there && !P.zero_rest) return;
         const size_t slot0 = (size_t)pair * P.n_splits * P.rows + row;
         // Eight pieces' loads at a time: a few rows are all there is to hide their latency.
         constexpr int U = 8;
@@ -746,7 +762,7 @@ __global__ void __launch_bounds__(256) ffa_tree_finish_kernel(const TreeParams P
             }
         }
         T* to = static_cast<T*>(P.out) + b * P.out_stride[0] + (long long)(h * P.G + row % P.G) * P.out_stride[1] + token * P.out_stride[2];
-        store_out4(to + d, o / L);
+        store_out4(to + d, there ? o / L : f32x4_t{0.f, 0.f, 0.f, 0.f});
         return;
     }
     const int block = blockIdx.x - join_blocks;
@@ -769,7 +785,7 @@ __global__ void __launch_bounds__(256) ffa_tree_finish_kernel(const TreeParams P
 // ---------------------------------------------------------------------------------------
 template <typename T, int DH, int RT, int W> int launch_tree_kernel(const TreeParams& P, hipStream_t st) {
     const dim3 grid(8u * (unsigned)P.row_blocks, (unsigned)((P.B * P.H * P.n_splits + 7) / 8));
-    const size_t lds = (size_t)(tree_merge_floats<DH, W>() + P.rows * P.score_lds) * sizeof(float);
+    const size_t lds = (size_t)(tree_merge_floats<DH, W>() + tree_q_floats<T, DH, RT>() + P.rows * P.score_lds) * sizeof(float);
     hipLaunchKernelGGL((ffa_tree_kernel<T, DH, RT, W>), grid, dim3(W * 64), lds, st, TREE_HOT_OF(P), P);
     return hipGetLastError() == hipSuccess ? FFA_OK : FFA_ERR_LAUNCH;
 }

@@ -151,8 +151,7 @@ torch::Tensor attention_tree(torch::Tensor q, torch::Tensor k, torch::Tensor v, 
     const torch::Tensor cnt = int_input(counts, k_cache, {d.B}, "counts");
     // Token-major in memory, so that [B, n, Hq * Dh] is a view; rows past a sample's count are zero.
     const int64_t Hq = q.size(1);
-    torch::Tensor out = (cnt.defined() ? torch::zeros({d.B, n, Hq, d.Dh}, q.options())
-                                       : torch::empty({d.B, n, Hq, d.Dh}, q.options())).transpose(1, 2);
+    torch::Tensor out = torch::empty({d.B, n, Hq, d.Dh}, q.options()).transpose(1, 2);
     ffa_tree_tokens tt = {};
     tt.tokens = (int)n;
     tt.q_head_num = (int)Hq;
@@ -160,6 +159,7 @@ torch::Tensor attention_tree(torch::Tensor q, torch::Tensor k, torch::Tensor v, 
     tt.first_keys = int_ptr(fk);
     tt.lengths = int_ptr(len);
     tt.counts = int_ptr(cnt);
+    tt.zero_rest = 1;
     for (int i = 0; i < 3; ++i) {
         tt.q_stride[i] = q.stride(i);
         tt.k_stride[i] = k.stride(i);

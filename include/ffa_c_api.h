@@ -319,8 +319,9 @@ int ffa_load_floor(int precision, int batch_size, int head_num, int head_dim, in
  *   q_head_num  a multiple G * head_num of the cache's heads: query head hq reads head hq / G;
  *   parents     [B, tokens]: the node's parent, a node before it; any value outside [0, i) makes
  *               node i a child of the last cached token.  NULL: a chain;
- *   counts      [B]: sample b has only this many nodes (clamped to [0, tokens]); rows of `out`
- *               and cache slots of the others stay as they were.  NULL: all;
+ *   counts      [B]: sample b has only this many nodes (clamped to [0, tokens]); the cache slots of
+ *               the others stay as they were, their rows of `out` too, or are zero if zero_rest != 0.
+ *               NULL: all;
  *   *_stride    element strides of (sample, head, token) of q, k, v and out; each row of
  *               head_dim elements is contiguous, strides are multiples of 16 bytes, and the token
  *               strides of k and v are not negative and below 64 MiB.
@@ -338,6 +339,7 @@ typedef struct ffa_tree_tokens {
     const int32_t* first_keys;
     const int32_t* lengths;
     const int32_t* counts;
+    int32_t zero_rest;
     int64_t q_stride[3];
     int64_t k_stride[3];
     int64_t v_stride[3];

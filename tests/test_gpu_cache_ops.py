@@ -545,3 +545,29 @@ def test_refusals(what):
         bad(F.evict, [(kc, vc)], [w], 20, 5, 1, into=[(kc, kc.view(2, 2, -1, 64), w)])  # V into K's buffer
         F.evict([(kc, vc)], [w], 20, 5, 1, into=[(kc, other, w)])
     torch.cuda.synchronize()
+
+
+def test_rows_past_the_count_stay_as_they_were():
+    """Through the C ABI, which writes only what is there unless it is asked for zeros; one piece and several."""
+    import ctypes as C
+    from fastforwardattention_amd import capi
+    lib = capi.load()
+    for t in (50, 9000):
+        _, kc, vc, q, k, v = make(80, "fp16", 1, 2, 2, 64, t, 6)
+        counts, K0 = ints([4]), kc.clone()
+        for zero in (0, 1):
+            out = torch.full((1, 6, 2, 64), 7.0, dtype=torch.float16, device=DEV).transpose(1, 2)
+            tok = capi.TreeTokens()
+            tok.tokens, tok.q_head_num, tok.counts, tok.zero_rest = 6, 2, counts.data_ptr(), zero
+            for name, x in (("q_stride", q), ("k_stride", k), ("v_stride", v), ("out_stride", out)):
+                getattr(tok, name)[:] = x.stride()[:3]
+            n = lib.ffa_tree_workspace_bytes(16, 1, 2, 2, 64, 6, t)
+            ws = torch.empty(n + 1, dtype=torch.uint8, device=DEV)
+            p = [C.c_void_p(x.data_ptr()) for x in (q, k, v, kc, vc, out, ws)]
+            rc = lib.ffa_attention_tree(16, 1, 2, 64, kc.shape[3], 0.125, t, C.byref(tok), *p, n, C.c_void_p(torch.cuda.current_stream().cuda_stream))
+            assert rc == capi.FFA_OK
+            torch.cuda.synchronize()
+            assert bool((out[:, :, 4:] == (0.0 if zero else 7.0)).all()) and not bool((out[:, :, :4] == 7.0).any())
+            want = FFA().attention_tree(q, k, v, kc, vc, 0.125, t, counts=counts)
+            assert torch.equal(out[:, :, :4], want[:, :, :4])
+            assert bool(kc[:, :, :, t + 4:].isnan().all()) and torch.equal(kc[:, :, :, :t], K0[:, :, :, :t])
