@@ -248,6 +248,14 @@ int ffa_commit_tree(int precision, int n_caches, void* const* k_caches, void* co
         if (!k_caches[i] || !v_caches[i]) return FFA_ERR_NULL_POINTER;
         if (!aligned(k_caches[i], 16) || !aligned(v_caches[i], 16)) return FFA_ERR_ALIGNMENT;
     }
+    // A cache that is moved twice at once would be read behind its own writes.
+    const size_t bytes = (size_t)batch_size * head_num * max_seq_len * head_dim * elem_bytes(precision);
+    for (int i = 0; i < n_caches; ++i) {
+        if (overlap(k_caches[i], bytes, v_caches[i], bytes)) return FFA_ERR_OVERLAP;
+        for (int j = 0; j < i; ++j)
+            for (const void* a : {(const void*)k_caches[i], (const void*)v_caches[i]})
+                if (overlap(a, bytes, k_caches[j], bytes) || overlap(a, bytes, v_caches[j], bytes)) return FFA_ERR_OVERLAP;
+    }
     for (int i0 = 0; i0 < n_caches; i0 += kSlotCaches) {
         CommitParams P = {};
         P.n_caches = std::min(kSlotCaches, n_caches - i0);

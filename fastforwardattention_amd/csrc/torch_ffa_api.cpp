@@ -98,7 +98,9 @@ CacheDims checked_caches(const torch::Tensor& k_cache, const torch::Tensor& v_ca
     TORCH_CHECK(k_cache.is_cuda() && v_cache.is_cuda() && k_cache.device() == v_cache.device() &&
                     k_cache.scalar_type() == v_cache.scalar_type(),
                 "ff_attention: caches must be GPU tensors of one dtype on one device");
-    return dims_of(k_cache, v_cache);
+    const CacheDims d = dims_of(k_cache, v_cache);
+    TORCH_CHECK(d.B > 0 && d.H > 0 && d.Lmax > 0 && d.Dh > 0, "ff_attention: empty caches");
+    return d;
 }
 
 // An int32 tensor of `shape` on the caches' device; empty = not given.

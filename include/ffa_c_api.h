@@ -57,8 +57,8 @@ typedef enum ffa_status {
                                 /* cache's heads, or a stride that is no multiple of 16 bytes */
     FFA_ERR_EVICT = 17,         /* eviction: keep < 1 or past the target, recent outside      */
                                 /* [0, keep]                                                  */
-    FFA_ERR_OVERLAP = 18        /* eviction: a target overlaps another buffer of the call and */
-                                /* is not exactly its own source                              */
+    FFA_ERR_OVERLAP = 18        /* two caches of a commit overlap, or an eviction's target    */
+                                /* overlaps another buffer and is not exactly its own source  */
 } ffa_status;
 
 /* precision codes: the same integers the reference passes to get_launch_params
@@ -361,7 +361,8 @@ int ffa_attention_tree(int precision, int batch_size, int head_num, int head_dim
  * larger than the one before); accepted [B] is clamped to [0, path_len], a node to
  * [0, FFA_MAX_TREE_TOKENS - 1] and to the cache.
  * All old slots of a sample are read before any is written, so that every path is a gather.
- * path_len 1 .. FFA_MAX_TREE_TOKENS; k_caches and v_caches are HOST arrays of device pointers.
+ * path_len 1 .. FFA_MAX_TREE_TOKENS; k_caches and v_caches are HOST arrays of device pointers to
+ * buffers that do not overlap.
  */
 int ffa_commit_tree(int precision, int n_caches, void* const* k_caches, void* const* v_caches,
                     int batch_size, int head_num, int head_dim, int max_seq_len, int t,

@@ -57,6 +57,11 @@ def test_tree_refusals(lib):
         bad = tokens()
         getattr(bad, name)[1] = 68
         assert tree(lib, tok=bad) == capi.FFA_ERR_TREE
+    for name in ("k_stride", "v_stride"):
+        for step in (-64, (1 << 26) // 2):
+            bad = tokens()
+            getattr(bad, name)[2] = step
+            assert tree(lib, tok=bad) == capi.FFA_ERR_TREE
     # few pairs, a long cache: pieces, and so a workspace
     need = lib.ffa_tree_workspace_bytes(16, 1, 1, 1, 64, 4, 5000)
     one = tokens(Hq=1, H=1)
@@ -109,6 +114,10 @@ def test_commit_refusals(lib):
     assert call(v=pointers(0x200008)) == capi.FFA_ERR_ALIGNMENT
     assert call(lengths=C.c_void_p(0x100002)) == capi.FFA_ERR_ALIGNMENT
     assert call(n=0) == capi.FFA_OK
+    # 2 x 4 x 128 slots of 128 bytes: 128 KiB a buffer
+    assert call(k=pointers(0x100000), v=pointers(0x110000)) == capi.FFA_ERR_OVERLAP
+    assert call(n=2, k=pointers(0x100000, 0x100000), v=pointers(0x200000, 0x300000)) == capi.FFA_ERR_OVERLAP
+    assert call(n=2, k=pointers(0x100000, 0x400000), v=pointers(0x200000, 0x11fff0)) == capi.FFA_ERR_OVERLAP
 
 
 def test_evict_refusals(lib):

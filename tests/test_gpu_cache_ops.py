@@ -164,6 +164,23 @@ def test_strides_and_alignment(dtype):
     run_tree(kc, vc, q, k[:, :1].expand(B, H, n, Dh), v[:, :1].expand(B, H, n, Dh), 0.125, t, dtype, "broadcast")
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1e-42, -1e-42])
+def test_scales_that_are_not_positive(dtype, scale):
+    """A negative scale turns the order of the keys, zero makes them all alike; masked keys stay masked."""
+    print("scale", dtype, scale, flush=True)
+    g, kc, vc, q, k, v = make(13, dtype, 2, 2, 4, 64, 130, 5)
+    run_tree(kc, vc, q, k, v, scale, 130, dtype, f"scale {scale}", parents=random_parents(g, 2, 5), first_keys=[0, 40], lengths=[130, 77])
+
+
+def test_far_apart_tokens_are_copied():
+    """A token stride of 64 MiB and more, in a buffer that holds it: the rows are brought together first."""
+    _, kc, vc, q, k, v = make(14, "fp16", 1, 1, 1, 64, 40, 2)
+    far = torch.empty(1 << 25 | 64, dtype=torch.float16, device=DEV).as_strided((1, 1, 2, 64), (1 << 25, 1 << 25, 1 << 25, 1))
+    far.copy_(k)
+    run_tree(kc, vc, q, far, v, 0.125, 40, "fp16", "far apart")
+
+
 def test_wrong_parents_mean_the_root():
     _, kc, vc, q, k, v = make(11, "fp16", 1, 2, 2, 64, 40, 6)
     run_tree(kc, vc, q, k, v, 0.125, 40, "fp16", "wrong parents", parents=torch.tensor([[7, 1, 1, -5, 3, 1 << 30]], dtype=torch.int32))
@@ -517,6 +534,7 @@ def test_refusals(what):
             bad(F.attention_tree, q, k, v, kc, vc, 1.0, 20, **{name: torch.zeros(3, dtype=torch.int32, device=DEV)})
             bad(F.attention_tree, q, k, v, kc, vc, 1.0, 20, **{name: torch.zeros((2, 4) if name == "parents" else 2, dtype=torch.int32)})
         bad(F.attention_tree, q, k, v, kc[:, :, :, ::2], vc[:, :, ::2], 1.0, 4)
+        bad(F.attention_tree, q, k[:, :0], v[:, :0], kc[:, :0].contiguous(), vc[:, :0].contiguous(), 1.0, 4)
     if what == "weights":
         bad(F.attention_weights, q1, k1, v1, kc, vc, 1.0, kc.shape[3], w)
         bad(F.attention_weights, q1, k1, v1, kc, vc, 1.0, 20, w[:, :, :-1])
@@ -531,6 +549,7 @@ def test_refusals(what):
         bad(F.commit_tree, [(kc, vc)], 20, path[:1], acc)
         bad(F.commit_tree, [(kc, vc)], 20, path, acc.cpu())
         bad(F.commit_tree, [(kc, vc), (kc.float(), vc.float())], 20, path, acc)
+        bad(F.commit_tree, [(kc, vc), (kc.clone(), vc)], 20, path, acc)                  # one cache twice
     if what == "evict":
         bad(F.evict, [(kc, vc)], [w], 20, 0, 0)
         bad(F.evict, [(kc, vc)], [w], 20, 5, 6)
