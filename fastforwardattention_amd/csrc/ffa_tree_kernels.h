@@ -564,13 +564,24 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT)) ffa_tree_
                 for (int j = 0; j < NJ; ++j) s[rt][j / 4][j % 4] = x[j];
             }
         }
+        // Turned ahead of the products, V leaves its registers to the next tile's loads: 8 % of a step over
+        // 1000 keys.  Where registers are short it costs more than that (four row tiles of Dh 128: -6 %).
+        constexpr bool EARLY = sizeof(T) == 2 && RT <= 2 && DH <= 128;
+        uint4 tv[EARLY ? NP : 1][EARLY ? DB : 1];
+        if constexpr (EARLY) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int q = 0; q < NP; ++q) tv[q][db] = vt.turned(q, db < G::NBLK * G::E ? db / G::E : G::NBLK, db < G::NBLK * G::E ? db % G::E : 0);
+            if (i + 1 < n_tiles) load_v(i + 1);
+        }
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
             const int blk = db < G::NBLK * G::E ? db / G::E : G::NBLK, e = db < G::NBLK * G::E ? db % G::E : 0;
             if constexpr (sizeof(T) == 2) {
 #pragma unroll
                 for (int q = 0; q < NP; ++q) {
-                    const uint4 a = vt.turned(q, blk, e);
+                    const uint4 a = EARLY ? tv[EARLY ? q : 0][EARLY ? db : 0] : vt.turned(q, blk, e);
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) {
                         acc[rt][db] = mma_qk(a, pf[rt][q].hi, acc[rt][db], T{});
@@ -585,7 +596,7 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT)) ffa_tree_
                         acc[rt][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(vt.at(j, blk, e), s[rt][j / 4][j % 4], acc[rt][db], 0, 0, 0);
             }
         }
-        if (i + 1 < n_tiles) load_v(i + 1);
+        if (!EARLY && i + 1 < n_tiles) load_v(i + 1);
     }
 
     // ---- join the waves: out = sum_w O_w 2^(m_w - M) / sum_w l_w 2^(m_w - M) ----
