@@ -74,9 +74,13 @@ struct PFrag16 { uint4 hi, lo; };
 typedef __fp16 fp16x2_t __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint32_t* lo, uint16_t) {
-    const half2_t h = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(a, b));
-    *hi = __builtin_bit_cast(uint32_t, h);
-    const half2_t rest = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float)h[0], -1.f, a), fmaf((float)h[1], -1.f, b)));
+    const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+    *hi = h;
+    // a - (lower half of h), b - (upper half): one instruction each, where the compiler converts first.
+    float ra, rb;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(h), "v"(a));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(h), "v"(b));
+    const half2_t rest = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(ra, rb));
     const half2_t tiny = __builtin_bit_cast(half2_t, 0x00010001u);  // 2^-24, the smallest fp16
     *lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(rest, tiny));
 }
