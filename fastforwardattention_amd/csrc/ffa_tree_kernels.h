@@ -725,82 +725,100 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT)) ffa_tree_
     }
 }
 
-// After the pieces.  The first join_blocks workgroups join the rows, four dims a thread:
-// out = sum_i O_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).  The others turn scores into weights: 256 keys of
-// a pair each.
+// After the pieces, a pair a grid row.  The first join_blocks workgroups of a pair join its rows, four
+// dims a thread: out = sum_i O_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).  The others turn scores into weights,
+// 1024 keys each.  Bound by latency (the partial results are a few MB at most): what the loads need comes
+// in the leading arguments, and eight pieces' loads are in flight at a time.
 struct RowTotal { float M, L; };
-__device__ __forceinline__ RowTotal row_total(const TreeParams& P, size_t slot0) {
-    RowTotal t = {-INFINITY, 0.f};
-    for (int s = 0; s < P.n_splits; ++s) t.M = fmaxf(t.M, P.ws_ml[(slot0 + (size_t)s * P.rows) * 2]);
-    for (int s = 0; s < P.n_splits; ++s) {
-        const float ms = P.ws_ml[(slot0 + (size_t)s * P.rows) * 2];
-        if (ms != -INFINITY) t.L += P.ws_ml[(slot0 + (size_t)s * P.rows) * 2 + 1] * __builtin_amdgcn_exp2f(ms - t.M);
+// By a whole wave: lane s takes pieces s and s + 64 (there are at most 128).
+__device__ __forceinline__ RowTotal row_total(const float* ws_ml, size_t slot0, int n_splits, int rows, int lane) {
+    float m[2], l[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int s = lane + 64 * i;
+        const size_t at = (slot0 + (size_t)min(s, n_splits - 1) * rows) * 2;
+        m[i] = s < n_splits ? ws_ml[at] : -INFINITY;
+        l[i] = s < n_splits ? ws_ml[at + 1] : 0.f;
     }
-    return t;
+    const float M = wave_max(fmaxf(m[0], m[1]));
+    float L = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) L += m[i] == -INFINITY ? 0.f : l[i] * __builtin_amdgcn_exp2f(m[i] - M);
+    return {M, wave_sum(L)};
 }
 
+constexpr int kFinishKeys = 4;  // keys a thread
+
 template <typename T, int DH>
-__global__ void __launch_bounds__(256) ffa_tree_finish_kernel(const TreeParams P, int join_blocks, int key_blocks) {
-    if ((int)blockIdx.x < join_blocks) {
-        const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-        const long long line = i / (DH / 4);
-        const int d = (int)(i % (DH / 4)) * 4;
-        if (line >= (long long)P.B * P.H * P.rows) return;
-        const int pair = (int)(line / P.rows), row = (int)(line % P.rows);
-        const int b = pair / P.H, h = pair % P.H, token = row / P.G;
-        const bool there = P.counts == nullptr || token < P.counts[b];
-        if (!there && !P.zero_rest) return;
-        const size_t slot0 = (size_t)pair * P.n_splits * P.rows + row;
-        // Eight pieces' loads at a time: a few rows are all there is to hide their latency.
-        constexpr int U = 8;
-        float M = -INFINITY, L = 0.f;
-        f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-        for (int s0 = 0; s0 < P.n_splits; s0 += U) {
-            float ms[U], ls[U];
-            f32x4_t os[U];
+__global__ void __launch_bounds__(256) ffa_tree_finish_kernel(const float* ws_acc, const float* ws_ml, int n_splits, int rows,
+                                                              int join_blocks, const TreeParams P) {
+    typedef float f32x2_t __attribute__((ext_vector_type(2)));
+    const int pairs = P.B * P.H;
+    for (int pair = blockIdx.y; pair < pairs; pair += gridDim.y) {
+        if ((int)blockIdx.x < join_blocks) {
+            const int i = blockIdx.x * 256 + threadIdx.x;
+            const int row = i / (DH / 4), d = i % (DH / 4) * 4;
+            if (row >= rows) return;
+            const size_t slot0 = (size_t)pair * n_splits * rows + row;
+            constexpr int U = 8;
+            float M = -INFINITY, L = 0.f;
+            f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+            for (int s0 = 0; s0 < n_splits; s0 += U) {
+                f32x2_t ml[U];
+                f32x4_t os[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const size_t slot = slot0 + (size_t)min(s0 + u, P.n_splits - 1) * P.rows;
-                ms[u] = P.ws_ml[slot * 2];
-                ls[u] = P.ws_ml[slot * 2 + 1];
-                os[u] = *reinterpret_cast<const f32x4_t*>(P.ws_acc + slot * DH + d);
-            }
-            float top = M;
+                for (int u = 0; u < U; ++u) {
+                    const size_t slot = slot0 + (size_t)min(s0 + u, n_splits - 1) * rows;
+                    ml[u] = *reinterpret_cast<const f32x2_t*>(ws_ml + slot * 2);
+                    os[u] = *reinterpret_cast<const f32x4_t*>(ws_acc + slot * DH + d);
+                }
+                float top = M;
 #pragma unroll
-            for (int u = 0; u < U; ++u) top = s0 + u < P.n_splits ? fmaxf(top, ms[u]) : top;
-            if (M != -INFINITY) {
-                const float f = __builtin_amdgcn_exp2f(M - top);
-                L *= f;
-                o *= f;
-            }
-            M = top;
+                for (int u = 0; u < U; ++u) top = s0 + u < n_splits ? fmaxf(top, ml[u].x) : top;
+                const float back = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
+                L = M == -INFINITY ? 0.f : L * back;
+                o = M == -INFINITY ? f32x4_t{0.f, 0.f, 0.f, 0.f} : o * back;
+                M = top;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (s0 + u >= P.n_splits || ms[u] == -INFINITY) continue;
-                const float f = __builtin_amdgcn_exp2f(ms[u] - M);
-                L += ls[u] * f;
-                o += os[u] * f;
+                for (int u = 0; u < U; ++u) {
+                    const bool counts = s0 + u < n_splits && ml[u].x != -INFINITY;
+                    const float f = counts ? __builtin_amdgcn_exp2f(ml[u].x - M) : 0.f;
+                    L += counts ? ml[u].y * f : 0.f;
+                    o += counts ? os[u] * f : f32x4_t{0.f, 0.f, 0.f, 0.f};
+                }
             }
+            const int b = quotient(pair, P.H, P.H_magic), h = pair - b * P.H, token = quotient(row, P.G, P.G_magic);
+            const bool there = P.counts == nullptr || token < P.counts[b];
+            if (there || P.zero_rest) {
+                T* to = static_cast<T*>(P.out) + b * P.out_stride[0] + (long long)(h * P.G + row - token * P.G) * P.out_stride[1] + token * P.out_stride[2];
+                store_out4(to + d, there ? o / L : f32x4_t{0.f, 0.f, 0.f, 0.f});
+            }
+            continue;
         }
-        T* to = static_cast<T*>(P.out) + b * P.out_stride[0] + (long long)(h * P.G + row % P.G) * P.out_stride[1] + token * P.out_stride[2];
-        store_out4(to + d, there ? o / L : f32x4_t{0.f, 0.f, 0.f, 0.f});
-        return;
+        int first, length;
+        sample_range(P.first_keys, P.lengths, quotient(pair, P.H, P.H_magic), P.t, &first, &length);
+        const int j0 = (blockIdx.x - join_blocks) * 256 * kFinishKeys + threadIdx.x;
+        float w[kFinishKeys] = {};
+        for (int row = 0; row < rows; ++row) {
+            const float* x = P.ws_scores + ((size_t)pair * rows + row) * P.score_stride;
+            float z[kFinishKeys];
+#pragma unroll
+            for (int k = 0; k < kFinishKeys; ++k) {
+                const int j = j0 + k * 256;
+                z[k] = j > length || j < first ? -INFINITY : x[j == length ? P.score_stride - 64 : j];
+            }
+            const RowTotal t = row_total(ws_ml, (size_t)pair * n_splits * rows + row, n_splits, rows, threadIdx.x & 63);
+#pragma unroll
+            for (int k = 0; k < kFinishKeys; ++k) w[k] += __builtin_amdgcn_exp2f(z[k] - t.M) / t.L;
+        }
+#pragma unroll
+        for (int k = 0; k < kFinishKeys; ++k) {
+            const int j = j0 + k * 256;
+            float* to = P.key_weights + (size_t)pair * P.Lmax + j;
+            if (j == length) *to = w[k];
+            else if (j < length && j >= first) *to += w[k];
+        }
     }
-    const int block = blockIdx.x - join_blocks;
-    const int pair = block / key_blocks, b = pair / P.H;
-    int first, length;
-    sample_range(P.first_keys, P.lengths, b, P.t, &first, &length);
-    const int j = (block % key_blocks) * 256 + threadIdx.x;
-    if (j > length || j < first) return;
-    float w = 0.f;
-    for (int row = 0; row < P.rows; ++row) {
-        const RowTotal t = row_total(P, (size_t)pair * P.n_splits * P.rows + row);
-        const float* x = P.ws_scores + ((size_t)pair * P.rows + row) * P.score_stride;
-        w += __builtin_amdgcn_exp2f(x[j == length ? P.score_stride - 64 : j] - t.M) / t.L;
-    }
-    float* to = P.key_weights + (size_t)pair * P.Lmax + j;
-    if (j == length) *to = w;
-    else *to += w;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -836,11 +854,10 @@ template <typename T, int DH> int launch_tree_dh(const TreeParams& P, const Tree
     if (rc != FFA_OK) return rc;
     const bool weights = P.ws_scores != nullptr && (P.n_splits > 1 || P.score_lds == 0);
     if (P.n_splits > 1 || weights) {
-        const long long threads = P.n_splits > 1 ? (long long)P.B * P.H * P.rows * (DH / 4) : 0;
-        const int join_blocks = (int)((threads + 255) / 256), key_blocks = (P.t + 1 + 255) / 256;
-        const long long blocks = join_blocks + (weights ? (long long)P.B * P.H * key_blocks : 0);
-        if (blocks > 0x7fffffffll) return FFA_ERR_SHAPE;
-        hipLaunchKernelGGL((ffa_tree_finish_kernel<T, DH>), dim3((unsigned)blocks), dim3(256), 0, st, P, join_blocks, key_blocks);
+        const int join_blocks = P.n_splits > 1 ? (int)(((long long)P.rows * (DH / 4) + 255) / 256) : 0;
+        const int key_blocks = weights ? (P.t + 256 * kFinishKeys) / (256 * kFinishKeys) : 0, pairs = P.B * P.H;
+        const dim3 grid((unsigned)(join_blocks + key_blocks), (unsigned)(pairs < 65535 ? pairs : 65535));
+        hipLaunchKernelGGL((ffa_tree_finish_kernel<T, DH>), grid, dim3(256), 0, st, P.ws_acc, P.ws_ml, P.n_splits, P.rows, join_blocks, P);
         if (hipGetLastError() != hipSuccess) return FFA_ERR_LAUNCH;
     }
     return FFA_OK;

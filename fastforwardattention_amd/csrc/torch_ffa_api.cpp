@@ -125,6 +125,7 @@ torch::Tensor group_input(const torch::Tensor& x, const torch::Tensor& like, con
 }
 
 torch::Tensor scratch(size_t bytes, const torch::Tensor& like) {
+    if (bytes == 0) return torch::Tensor();
     return torch::empty({(int64_t)bytes}, torch::TensorOptions().dtype(torch::kUInt8).device(like.device()));
 }
 
