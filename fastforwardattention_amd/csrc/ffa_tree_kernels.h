@@ -268,8 +268,9 @@ template <typename T, int DH, int RT> constexpr int tree_q_floats() {
                        (int)((P).lengths != nullptr || (P).first_keys != nullptr)
 
 // STREAM: the caches are read once and go past the L2's replacement order, worth 13 % of a step over 1 GB.
-// Not where several row blocks read the same keys (96 rows in two blocks, 20000 keys, Dh 128: 57 us
-// streamed, 50 us not; 64 rows of Dh 256 in two blocks, 256 pairs of 8000 keys: 585 and 510 us).
+// Not where several row blocks read the same keys (64 rows of Dh 256 in two blocks, 256 pairs of 8000
+// keys: 585 us streamed, 548 us not; 96 rows of Dh 128 in two blocks, 16 pairs of 20000 keys: alike from
+// HBM, 57 and 50 us where the last-level cache holds the keys).
 template <typename T, int DH, int RT, int W, bool STREAM>
 __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT)) ffa_tree_kernel(TREE_HOT_DECL, const TreeParams P) {
     using G = TreeGeo<T, DH, RT>;
