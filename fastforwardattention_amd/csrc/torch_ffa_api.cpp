@@ -154,7 +154,7 @@ torch::Tensor attention_tree(torch::Tensor q, torch::Tensor k, torch::Tensor v, 
     const torch::Tensor cnt = int_input(counts, k_cache, {d.B}, "counts");
     // Token-major in memory, so that [B, n, Hq * Dh] is a view; rows past a sample's count are zero.
     const int64_t Hq = q.size(1);
-    torch::Tensor out = torch::empty({d.B, n, Hq, d.Dh}, q.options()).transpose(1, 2);
+    torch::Tensor out = at::empty_strided({d.B, Hq, n, d.Dh}, {n * Hq * d.Dh, d.Dh, Hq * d.Dh, 1}, q.options());
     ffa_tree_tokens tt = {};
     tt.tokens = (int)n;
     tt.q_head_num = (int)Hq;
