@@ -590,3 +590,40 @@ def test_rows_past_the_count_stay_as_they_were():
             want = FFA().attention_tree(q, k, v, kc, vc, 0.125, t, counts=counts)
             assert torch.equal(out[:, :, :4], want[:, :, :4])
             assert bool(kc[:, :, :, t + 4:].isnan().all()) and torch.equal(kc[:, :, :, :t], K0[:, :, :, :t])
+
+
+def test_caches_of_more_than_four_gigabytes():
+    """Offsets beyond 32 bits: the last pair's results against its own slots, in all four operators."""
+    B, H, Dh, t, n = 2, 16, 128, 590_000, 5
+    Lmax = t + 16
+    g = torch.Generator(device=DEV).manual_seed(90)
+    kc = torch.empty(B, H, Dh // 8, Lmax, 8, dtype=torch.float16, device=DEV).normal_(generator=g)
+    vc = torch.empty(B, H, Lmax, Dh, dtype=torch.float16, device=DEV).normal_(generator=g)
+    assert kc.numel() * 2 > 4 << 30
+    q, k, v = (torch.empty(B, H, n, Dh, dtype=torch.float16, device=DEV).normal_(generator=g) for _ in range(3))
+    last = slice(B - 1, B)
+    K0, V0 = unpack_k(kc[last, -1:])[:, :, :t].clone(), vc[last, -1:, :t].clone()
+    out = FFA().attention_tree(q, k, v, kc, vc, 0.05, t)
+    want, size, bound, _ = tree_reference(q[last, -1:], k[last, -1:], v[last, -1:], K0, V0, 0.05, t)
+    assert_close(out[last, -1:], want, tree_tolerance(q.dtype, want, size, bound, t + n, Dh), "long tree")
+    assert torch.equal(unpack_k(kc[last, -1:])[:, :, t:t + n], k[last, -1:]) and torch.equal(vc[last, -1:, t:t + n], v[last, -1:])
+    FFA().commit_tree([(kc, vc)], t, ints([[1, 4]] * B), ints([2] * B))
+    assert torch.equal(vc[last, -1:, t:t + 2], v[last, -1:, [1, 4]].view(1, 1, 2, Dh))
+    w = torch.rand(B, H, Lmax, generator=g, device=DEV)
+    w0 = w[-1, -1].double()
+    K1, V1 = unpack_k(kc[last, -1:])[:, :, :t + 2].clone(), vc[last, -1:, :t + 2].clone()
+    out = FFA().attention_weights(q[:, :, 0].contiguous(), k[:, :, 0].contiguous(), v[:, :, 0].contiguous(), kc, vc, 0.05, t + 2, w)
+    want, size, bound, p = tree_reference(q[last, -1:, :1], k[last, -1:, :1], v[last, -1:, :1], K1, V1, 0.05, t + 2)
+    assert_close(out[last, -1:, None], want, tree_tolerance(q.dtype, want, size, bound, t + 3, Dh), "long weights")
+    w0[:t + 2] += p[0][0, 0, 0, :-1]
+    w0[t + 2] = p[0][0, 0, 0, -1]
+    assert float((w[-1, -1, :t + 3].double() - w0[:t + 3]).abs().max()) <= 2.0 ** -23
+    keep = t - 1000
+    before = (unpack_k(kc[last, -1:])[0, 0].clone(), vc[-1, -1].clone(), w[-1, -1].clone())
+    kept = FFA().evict([(kc, vc)], [w], t + 3, keep, 64)[0, -1, -1].long()
+    rank = before[2][:t + 3].double()
+    rank[t + 3 - 64:] = math.inf
+    order = torch.sort(rank, descending=True, stable=True).indices[:keep].sort().values
+    assert torch.equal(kept, order)
+    assert torch.equal(unpack_k(kc[last, -1:])[0, 0, :keep], before[0][order]) and torch.equal(vc[-1, -1, :keep], before[1][order])
+    assert torch.equal(w[-1, -1, :keep], before[2][order])
