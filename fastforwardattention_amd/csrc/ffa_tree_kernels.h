@@ -708,13 +708,30 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT)) ffa_tree_
     if (weights && P.score_lds != 0) {
         const int from = max(first, piece0), to = min(length, piece0 + tiles_per_split * TK);
         if (whole) {
+            // Eight keys a thread and step: their sums are on the way while the weights are formed.
             float* kw = P.key_weights + (size_t)pair * Lmax;
-            for (int j = from + tid; j <= to; j += W * 64) {
-                float w = 0.f;
-                for (int r = 0; r < P.rows; ++r)
-                    w += __builtin_amdgcn_exp2f(s_scores[r * P.score_lds + (j == length ? P.score_lds - 64 : j - piece0)] - s_row[r][0]) / s_row[r][1];
-                if (j == length) kw[j] = w;
-                else kw[j] += w;
+            constexpr int U = 8;
+            for (int j0 = from + tid; j0 <= to; j0 += U * W * 64) {
+                float sum[U], w[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    sum[u] = kw[min(j0 + u * W * 64, to)];
+                    w[u] = 0.f;
+                }
+                for (int r = 0; r < P.rows; ++r) {
+                    const float M = s_row[r][0], per = 1.f / s_row[r][1];
+                    const float* x = s_scores + r * P.score_lds;
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int j = min(j0 + u * W * 64, to);
+                        w[u] += __builtin_amdgcn_exp2f(x[j == length ? P.score_lds - 64 : j - piece0] - M) * per;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int j = j0 + u * W * 64;
+                    if (j <= to) kw[j] = j == length ? w[u] : sum[u] + w[u];
+                }
             }
         } else {
             for (int r = 0; r < P.rows; ++r) {
