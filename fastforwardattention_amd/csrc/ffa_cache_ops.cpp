@@ -128,6 +128,9 @@ size_t tree_workspace(int precision, int B, int H, int Hq, int Dh, int tokens, i
     return tree_sizes(B * H, (int)rows, Dh, n, scores, t).total();
 }
 
+// Caches of a launch: a grid has fewer than 2^32 threads in x, and its workgroups up to 1024 a pair and cache.
+int launch_caches(long long pairs) { return (int)std::min<long long>(kSlotCaches, (1ll << 21) / pairs); }
+
 bool overlap(const void* a, size_t na, const void* b, size_t nb) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
     return x < y + nb && y < x + na;
@@ -256,9 +259,10 @@ int ffa_commit_tree(int precision, int n_caches, void* const* k_caches, void* co
             for (const void* a : {(const void*)k_caches[i], (const void*)v_caches[i]})
                 if (overlap(a, bytes, k_caches[j], bytes) || overlap(a, bytes, v_caches[j], bytes)) return FFA_ERR_OVERLAP;
     }
-    for (int i0 = 0; i0 < n_caches; i0 += kSlotCaches) {
+    const int most = launch_caches((long long)batch_size * head_num);
+    for (int i0 = 0; i0 < n_caches; i0 += most) {
         CommitParams P = {};
-        P.n_caches = std::min(kSlotCaches, n_caches - i0);
+        P.n_caches = std::min(most, n_caches - i0);
         for (int i = 0; i < P.n_caches; ++i) {
             P.k[i] = k_caches[i0 + i];
             P.v[i] = v_caches[i0 + i];
@@ -312,9 +316,10 @@ int ffa_evict(int precision, int n_caches, const void* const* k_src, const void*
             if (overlap(dst[a], na, kept, (size_t)n_caches * pairs * keep * 4)) return FFA_ERR_OVERLAP;
         }
     }
-    for (int i0 = 0; i0 < n_caches; i0 += kSlotCaches) {
+    const int most = launch_caches((long long)pairs);
+    for (int i0 = 0; i0 < n_caches; i0 += most) {
         EvictParams P = {};
-        P.n_caches = std::min(kSlotCaches, n_caches - i0);
+        P.n_caches = std::min(most, n_caches - i0);
         for (int i = 0; i < P.n_caches; ++i) {
             P.k_src[i] = k_src[i0 + i]; P.v_src[i] = v_src[i0 + i]; P.w_src[i] = w_src[i0 + i];
             P.k_dst[i] = k_dst[i0 + i]; P.v_dst[i] = v_dst[i0 + i]; P.w_dst[i] = w_dst[i0 + i];

@@ -277,26 +277,28 @@ __global__ void __launch_bounds__(NW * 64) ffa_evict_select_kernel(const EvictPa
     }
 }
 
-// Eviction, second kernel: the rows of K and V.  One wave takes one chunk row of a pair's K (64
+// Eviction, second kernel: the rows of K and V.  W waves take one chunk row of a pair's K (64
 // slots of 16 bytes an access) or one column block of its V (128 bytes a slot) through the kept slots
-// of its segment in order.  In place there is one segment, and nothing else to synchronise: kept[j] >= j,
-// so what is stored for slots [j, j + n) can only overwrite sources of entries before j + n, which this
-// wave has loaded already, and no other wave touches the column.  Two batches of loads are in flight.
+// in order, a batch of W * 8 accesses at a time, the next one's loads in flight.  Where targets and sources are
+// apart nothing orders the waves: W is 1, and a column is cut into segments.  In place, kept[j] >= j: what is
+// stored for slots [j, j + n) can only overwrite sources of entries before j + n, so a batch is stored once
+// all waves have its loads, and the loads of the next batch, whose sources are at j + n and after, need not wait
+// for those stores.  No other workgroup touches the column.
 // Bound by the memory: K is read in whole 128-byte lines of 8 slots, of which a random choice of slots
 // leaves few out.
 constexpr int kMoveBatch = 8;  // accesses of a batch
 
-template <int NCH>
-__global__ void __launch_bounds__(256) ffa_evict_move_kernel(const EvictParams P) {
+template <int NCH, int W>
+__global__ void __launch_bounds__(W == 1 ? 256 : W * 64) ffa_evict_move_kernel(const EvictParams P) {
     constexpr int NB = Columns<NCH>::NB, COLS = Columns<NCH>::COLS, RPI = Columns<NCH>::RPI, U = kMoveBatch;
     const int lane = threadIdx.x & 63;
-    const unsigned unit = blockIdx.x * 4 + wave_of_four();
-    const int pairs = P.B * P.H;
-    constexpr int UNITS = NCH + COLS;
-    const int col = (int)(unit % UNITS);
-    const unsigned rest = unit / UNITS;
-    const int pair = (int)(rest % pairs), cache = (int)(rest / pairs);
-    if (cache >= P.n_caches) return;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int pairs = P.B * P.H, cache = blockIdx.z;
+    constexpr unsigned UNITS = NCH + COLS;
+    const unsigned unit = blockIdx.x * 4 + wave;  // W == 1
+    const int col = W == 1 ? (int)(unit % UNITS) : (int)blockIdx.y;
+    const int pair = W == 1 ? (int)(unit / UNITS) : (int)blockIdx.x;
+    if (pair >= pairs) return;
     const int b = pair / P.H;
     const int length = P.lengths ? min(max(P.lengths[b], 0), P.t) : P.t;
     const int stay = min(length, P.keep);
@@ -314,13 +316,14 @@ __global__ void __launch_bounds__(256) ffa_evict_move_kernel(const EvictParams P
         dst = static_cast<char*>(P.v_dst[cache]) + ((size_t)pair * P.dst_len * NCH + (col - NCH) * NB) * 16;
         step = NCH * 16; rows = RPI; r0 = lane / NB; lane_bytes = lane % NB * 16;
     }
-    const bool in_place = src == dst;
+    const bool in_place = W > 1 && src == dst;
     if (in_place && length <= P.keep) return;
     const int* kept = P.kept + ((size_t)cache * pairs + pair) * P.keep;
-    const int batch = U * rows;
-    // Segments are whole batches.
-    const int from0 = blockIdx.y * P.segment_batches * batch;
-    const int end = blockIdx.y + 1 == gridDim.y ? stay : min(stay, from0 + P.segment_batches * batch);
+    const int batch = W * U * rows;
+    if (W > 1) r0 += wave * rows;
+    // Segments (W == 1) are whole batches.
+    const int from0 = W == 1 ? blockIdx.y * P.segment_batches * batch : 0;
+    const int end = W > 1 || blockIdx.y + 1 == gridDim.y ? stay : min(stay, from0 + P.segment_batches * batch);
     if (from0 >= end) return;
 
     int from[2][U];
@@ -328,14 +331,14 @@ __global__ void __launch_bounds__(256) ffa_evict_move_kernel(const EvictParams P
     unsigned moved[2] = {0, 0};  // bit u: access u of the batch has a slot of this lane to store
     auto load_slots = [&](int s, int j0) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) from[s][u] = kept[min(j0 + u * rows + r0, end - 1)];
+        for (int u = 0; u < U; ++u) from[s][u] = kept[min(j0 + u * W * rows + r0, end - 1)];
     };
     auto load = [&](int s, int j0) {
         moved[s] = 0;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = j0 + u * rows + r0;
-            if (j < end && (is_k || r0 < RPI) && !(in_place && from[s][u] == j)) moved[s] |= 1u << u;
+            const int j = j0 + u * W * rows + r0;
+            if (j < end && (is_k || lane < RPI * NB) && !(in_place && from[s][u] == j)) moved[s] |= 1u << u;
         }
         if (__any(moved[s] != 0)) {
 #pragma unroll
@@ -346,10 +349,16 @@ __global__ void __launch_bounds__(256) ffa_evict_move_kernel(const EvictParams P
         }
     };
     auto store = [&](int s, int j0) {
+        if (W > 1) {
+            // The uses make the wave wait for this batch before it says so.
+#pragma unroll
+            for (int u = 0; u < U; ++u) asm volatile("" : "+v"(x[s][u]));
+            __syncthreads();
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (moved[s] >> u & 1) {
-                const size_t at = (size_t)(j0 + u * rows + r0) * step + lane_bytes;
+                const size_t at = (size_t)(j0 + u * W * rows + r0) * step + lane_bytes;
                 __builtin_nontemporal_store(x[s][u], reinterpret_cast<u32x4_t*>(dst + at));
             }
     };
@@ -398,18 +407,29 @@ template <int NCH> static int evict_nch(EvictParams P, hipStream_t st) {
     else if (P.t <= held_slots(16, 8)) hipLaunchKernelGGL((ffa_evict_select_kernel<16, 8>), grid, dim3(16 * 64), 0, st, P);
     else hipLaunchKernelGGL((ffa_evict_select_kernel<16, 0>), grid, dim3(16 * 64), 0, st, P);
     if (launched() != FFA_OK) return FFA_ERR_LAUNCH;
-    const long long units = lines * (NCH + Columns<NCH>::COLS);
-    // In place a column is one wave's.  Otherwise columns are cut where their waves would leave the chip
-    // half empty, down to one batch.
+    constexpr int UNITS = NCH + Columns<NCH>::COLS;
     bool in_place = false;
     for (int i = 0; i < P.n_caches; ++i) in_place = in_place || P.k_src[i] == P.k_dst[i] || P.v_src[i] == P.v_dst[i];
-    const int stay = P.t < P.keep ? P.t : P.keep;
+    const int pairs = P.B * P.H, stay = P.t < P.keep ? P.t : P.keep;
+    // In place: a column is one workgroup's, of 8 waves, or of 4 for few slots, where half of 8 would have none
+    // of K's (us of the operator with 1, 4 and 8 waves, bf16: 8x32x128, 1000 of 1100 slots 71.0, 62.8, 64.7;
+    // 1x32x64, 512 of 600 12.4, 9.5, 10.6; 8x32x128, 2048 of 4096 168, 146, 140; 1x8x128, 4283 of 5873 55.4, 27.0,
+    // 24.6; 16 waves 25.5 there and 103 at 1000 of 1100).
+    if (in_place) {
+        const dim3 columns((unsigned)pairs, UNITS, (unsigned)P.n_caches);
+        if (stay <= 1024) hipLaunchKernelGGL((ffa_evict_move_kernel<NCH, 4>), columns, dim3(256), 0, st, P);
+        else hipLaunchKernelGGL((ffa_evict_move_kernel<NCH, 8>), columns, dim3(512), 0, st, P);
+        return launched();
+    }
+    // Otherwise columns are cut where their waves would leave the chip half empty, down to one batch.
+    const long long units = lines * UNITS;
     const int batches = (stay + kMoveBatch * Columns<NCH>::RPI - 1) / (kMoveBatch * Columns<NCH>::RPI);  // of V: K's hold more
-    long long segments = in_place ? 1 : (8192 + units - 1) / units;
+    long long segments = (8192 + units - 1) / units;
     if (segments > batches) segments = batches < 1 ? 1 : batches;
     P.segment_batches = (int)((batches + segments - 1) / segments);
     if (P.segment_batches < 1) P.segment_batches = 1;
-    hipLaunchKernelGGL(ffa_evict_move_kernel<NCH>, dim3((unsigned)((units + 3) / 4), (unsigned)segments), dim3(256), 0, st, P);
+    hipLaunchKernelGGL((ffa_evict_move_kernel<NCH, 1>), dim3((unsigned)((pairs * UNITS + 3) / 4), (unsigned)segments, (unsigned)P.n_caches),
+                       dim3(256), 0, st, P);
     return launched();
 }
 

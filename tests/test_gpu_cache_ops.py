@@ -627,3 +627,32 @@ def test_caches_of_more_than_four_gigabytes():
     assert torch.equal(kept, order)
     assert torch.equal(unpack_k(kc[last, -1:])[0, 0, :keep], before[0][order]) and torch.equal(vc[-1, -1, :keep], before[1][order])
     assert torch.equal(w[-1, -1, :keep], before[2][order])
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_as_many_pairs_as_there_may_be(in_place):
+    """2^18 pairs in 33 caches: more threads than one launch can have."""
+    B, H, Dh, Lmax, layers = 1024, 256, 64, 2, 33
+    g = torch.Generator(device=DEV).manual_seed(91)
+    caches = [tuple(torch.empty(shape, dtype=torch.float16, device=DEV).normal_(generator=g)
+                    for shape in ((B, H, Dh // 8, Lmax, 8), (B, H, Lmax, Dh))) for _ in range(layers)]
+    weights = [torch.rand(B, H, Lmax, generator=g, device=DEV) for _ in range(layers)]
+    second = [w[..., 1] > w[..., 0] for w in weights]
+    want = [(torch.where(s[..., None, None], k[..., 1, :], k[..., 0, :]),
+             torch.where(s[..., None], v[..., 1, :], v[..., 0, :]), w.amax(-1)) for s, (k, v), w in zip(second, caches, weights)]
+    if in_place:
+        to, to_w = caches, weights
+        kept = FFA().evict(caches, weights, Lmax, 1, 0)
+    else:
+        to = [tuple(torch.zeros_like(x) for x in pair) for pair in caches]
+        to_w = [torch.zeros_like(w) for w in weights]
+        kept = FFA().evict(caches, weights, Lmax, 1, 0, into=[(k, v, w) for (k, v), w in zip(to, to_w)])
+    for i in range(layers):
+        assert torch.equal(kept[i, ..., 0], second[i].int())
+        assert torch.equal(to[i][0][..., 0, :], want[i][0]), i
+        assert torch.equal(to[i][1][..., 0, :], want[i][1]) and torch.equal(to_w[i][..., 0], want[i][2]), i
+    one = [tuple(x[..., 1, :].clone() for x in pair) for pair in caches]
+    FFA().commit_tree(caches, 0, ints([[1]] * B), ints([1] * B))
+    for pair, rows in zip(caches, one):
+        for x, row in zip(pair, rows):
+            assert torch.equal(x[..., 0, :], row) and torch.equal(x[..., 1, :], row)
