@@ -60,22 +60,33 @@ struct TreeShape {
     int row_tiles, row_blocks, tile_keys, most_splits;
 };
 
+// 16-row tiles a workgroup may hold: more read the keys less often, but leave fewer waves a SIMD and cost more
+// before the first key and after the last.  Measured, us with two and with four, fp16 (B x H x Dh, 64 rows):
+//   one, where all workgroups of one tile run at once: 1x32x128 t 1000 15 and 24 (2 pairs, 472 rows, Dh 256 one 14,
+//   two 21); two up to 1280 keys: 8x32x128 t 512 23 and 28, t 1000 38 and 40, t 2000 84 and 71;
+//   four of 16-bit Dh 64, two of whose workgroups fit a CU, where there are more: 16x32x64 t 0 17.7 and 14.1, t 600
+//   33 and 29, t 4000 150 and 103 (8x32x64 t 0 10.3 and 11.5);
+//   two of Dh 80, whose tiles take as many registers as Dh 96 would: 16x32x80 t 1000 52 and 69, 2x8(64) t 4000 35
+//   and 46, but 1x32 t 4000 33 and 25.
+int most_row_tiles(int precision, int head_dim, int t, long long tiles, int cus) {
+    const int most = tree_row_tiles(head_dim);
+    if (head_dim == 64 && elem_bytes(precision) == 2 && tiles > 4 * cus) return most;
+    if (t <= 1280) return tiles <= cus ? 1 : 2;
+    return head_dim == 80 && tiles > cus ? 2 : most;
+}
+
 // What does not depend on the cut of the keys.  most_splits grows with t.
 TreeShape tree_shape(int precision, int pairs, int rows, int head_dim, int t, int cus) {
     TreeShape s;
     const int row_tiles = ceil_div(rows, 16);
-    // On few keys a workgroup's fixed cost counts, which grows with its rows, more than reading the keys
-    // again (256 pairs, 64 rows, two and four row tiles, 0, 512, 2000 keys: Dh 128 12.4 and 16.6, 23.4 and 27.6,
-    // 84 and 71 us; Dh 64 9.6 and 10.7, 16.5 and 17.6, 38.3 and 37.6 us), and one row tile is best where all
-    // workgroups run at once (2 pairs, 472 rows, 267 keys, Dh 256: one 14, two 21 us).
-    const int few = pairs * row_tiles <= cus ? 1 : 2;
-    s.row_blocks = ceil_div(row_tiles, t <= 768 ? few : tree_row_tiles(head_dim));
+    s.row_blocks = ceil_div(row_tiles, most_row_tiles(precision, head_dim, t, (long long)pairs * row_tiles, cus));
     s.row_tiles = ceil_div(row_tiles, s.row_blocks);
     s.tile_keys = 16 * tree_tile_units(elem_bytes(precision), head_dim, s.row_tiles);
-    const int tiles = ceil_div(t, s.tile_keys), groups = pairs * s.row_blocks;
+    const int tiles = ceil_div(t, s.tile_keys);
+    const long long groups = (long long)pairs * s.row_blocks;
     // One workgroup a CU streams at the memory's rate (measured from 1/4 to 16 a CU: 8 heads x 20000 keys
     // 167, 95, 63, 84, 117 us at 1/4, 1/2, 1, 2, 4), more only add partial results to join.
-    const int most = std::max(1, std::min({ceil_div(cus, groups), tiles / 2, 128}));
+    const int most = std::max(1, std::min({(int)((cus + groups - 1) / groups), tiles / 2, 128}));
     s.most_splits = tiles - tiles / most < kJoinTiles ? 1 : most;
     return s;
 }
