@@ -656,3 +656,29 @@ def test_as_many_pairs_as_there_may_be(in_place):
     for pair, rows in zip(caches, one):
         for x, row in zip(pair, rows):
             assert torch.equal(x[..., 0, :], row) and torch.equal(x[..., 1, :], row)
+
+
+@pytest.mark.parametrize("t,keep", [(300, 200), (2500, 1700)])
+def test_evict_keys_in_place_and_values_apart(t, keep):
+    """One call with both: the keys stay in their cache, values and weights go to others."""
+    B, H, Dh = 2, 3, 80
+    g = torch.Generator(device=DEV).manual_seed(92)
+    kc = torch.empty(B, H, Dh // 8, t, 8, dtype=torch.float16, device=DEV).normal_(generator=g)
+    vc = torch.empty(B, H, t, Dh, dtype=torch.float16, device=DEV).normal_(generator=g)
+    w = torch.rand(B, H, t, generator=g, device=DEV)
+    lengths = ints([t, keep - 3])
+    K0, V0, W0 = unpack_k(kc).clone(), vc.clone(), w.clone()
+    v2, w2 = torch.full_like(vc, 7), torch.full_like(w, 7)
+    kept = FFA().evict([(kc, vc)], [w], t, keep, 20, lengths=lengths, into=[(kc, v2, w2)])[0].long()
+    assert torch.equal(vc, V0) and torch.equal(w, W0)
+    for b, n in enumerate((keep, keep - 3)):
+        assert bool((kept[b, :, n:] == -1).all())
+        for h in range(H):
+            order = kept[b, h, :n]
+            rank = W0[b, h, :int(lengths[b])].double()
+            rank[-20:] = math.inf
+            want = torch.sort(rank, descending=True, stable=True).indices[:n].sort().values
+            assert torch.equal(order, want)
+            assert torch.equal(unpack_k(kc)[b, h, :n], K0[b, h, order]) and torch.equal(v2[b, h, :n], V0[b, h, order])
+            assert torch.equal(w2[b, h, :n], W0[b, h, order])
+        assert bool((v2[b, :, n:] == 7).all()) and bool((w2[b, :, n:] == 7).all())
