@@ -30,7 +30,8 @@ Written against the installed transformers (5.x) instead of a patched copy of it
 
 * passes of several tokens after the prompt (a prompt in chunks, assisted and prompt-lookup
   decoding), which the reference's models cannot run, go to `attention_tree` as chains of up to 64
-  tokens; `crop` takes rejected tokens back.
+  tokens; `crop` takes rejected tokens back.  Their mask may hold left padding, also of more than the
+  first chunk, and causal order; any other is refused.
 * a cache of bounded size (`FFACache(..., keep=n, recent=m)`): every step goes to
   `attention_weights`, which sums the attention each key receives, starting from the prompt's own;
   whenever evict_every tokens have come on top of `keep`, `evict` keeps the last `recent` tokens
@@ -97,6 +98,7 @@ class FFALayer(CacheLayerMixin):
         self.seen = 0               # tokens so far: more than t once some were evicted
         self.max_len = 0
         self.first_key = None       # int32 [B]: first real key of each left-padded sample
+        self.max_first = 0          # its largest entry: t or more while a sample has no real key yet
         self._hooked = False        # the attention hook has seen this layer's prompt pass
         self._pending = False       # a decode token was handed out and not yet attended
 
@@ -141,6 +143,7 @@ class FFALayer(CacheLayerMixin):
 
     def reset(self):
         self.engine, self.t, self.max_len, self.first_key, self.beam_table = None, 0, 0, None, None
+        self.max_first = 0
         self.seen, self.bounded = 0, None
         self._hooked = self._pending = False
 
@@ -205,15 +208,62 @@ class FFALayer(CacheLayerMixin):
 
     def note_prompt_mask(self, attention_mask):
         """Left-padding offsets from the prompt pass's mask, as the reference takes them:
-        index of the first maximum of the last query row (modeling_opt.py:222)."""
+        index of the first maximum of the last query row (modeling_opt.py:222).  A sample whose last
+        row sees nothing is all padding so far: its first real key lies behind the prompt."""
         self._hooked = True
+        self.first_key, self.max_first = None, 0
         if attention_mask is None:
-            self.first_key = None
             return
         row = attention_mask[:, :, -1, :]
+        none = ~_visible(row).any(dim=-1)
         if row.dtype == torch.bool:
             row = row.to(torch.int8)
-        self.first_key = torch.max(row, dim=-1).indices.reshape(-1).to(torch.int32).contiguous()
+        first = torch.where(none, row.shape[-1], torch.max(row, dim=-1).indices)
+        self.first_key = first.reshape(-1).to(torch.int32).contiguous()
+        self.max_first = int(self.first_key.max())
+        if self.keep is not None and self.max_first >= self.t:
+            raise NotImplementedError("FFACache: a bounded cache wants a real token of every sample in the prompt")
+
+    def takes_group(self, n: int) -> bool:
+        """Whether a pass of n tokens goes to attend_group: several tokens, or a sample that has no real
+        key yet, so that the pass's mask has to say whether its token is one."""
+        return n > 1 or (self.t <= self.max_first and self.first_key is not None and self.bounded is None
+                         and self.beam_table is None and hasattr(self.engine, "attention_tree"))
+
+    def _note_group_mask(self, mask, n: int):
+        """Left-padding offsets from the mask [B,1,n,t+n] of a pass of n tokens; returns the tokens' parents
+        (None: a chain).  The engine attends to the keys from a sample's first real one up to the token
+        itself, so any other mask is refused; rows of padding may hold anything."""
+        if mask is None:
+            return None
+        B, T = self.engine.get_cache()[1].shape[0], self.t + n
+        fits = mask.dim() == 4 and mask.shape[0] in (1, B) and tuple(mask.shape[1:]) == (1, n, T)
+        if fits:
+            mask = mask[:, 0].expand(B, n, T)
+            key = torch.arange(T, device=mask.device)
+            last = _visible(mask[:, -1])
+            first = torch.where(last.any(dim=-1), torch.max(last.to(torch.int8), dim=-1).indices, T)
+            wrong = torch.zeros((), dtype=torch.bool, device=mask.device)
+            for i in range(0, n, 256):      # bounds the temporaries
+                part, at = mask[:, i:i + 256], key[None, self.t + i:self.t + min(n, i + 256), None]
+                seen, since = _visible(part), first[:, None, None]
+                differs = seen != ((key >= since) & (key <= at))
+                if part.dtype.is_floating_point:
+                    differs |= seen & (part != 0)       # a bias
+                wrong |= (differs & (at >= since)).any()
+            wrong, max_first = torch.stack([wrong.to(first.dtype), first.max()]).tolist()
+            fits = not wrong
+        if not fits:
+            self._pending = False
+            raise NotImplementedError("FFACache: a pass of several tokens wants a mask [B,1,n,keys] of left padding and causal "
+                                      "order, the same for all heads; trees, windows, biases and padding behind a sample's "
+                                      "first token are not supported")
+        self.first_key, self.max_first = first.to(torch.int32).contiguous(), int(max_first)
+        if self.max_first <= self.t:
+            return None
+        # A sample that begins within the pass: its first real token sees no padding.
+        node = torch.arange(n, device=mask.device)
+        return torch.where(node == first[:, None] - self.t, -1, node - 1).to(torch.int32)
 
     def note_prompt_weights(self, weights):
         """The prompt pass's attention weights [B,H,Lq,Lk], for a bounded cache: what each key received
@@ -239,18 +289,20 @@ class FFALayer(CacheLayerMixin):
             self.first_key = (self.first_key - gone).clamp_(min=0)
         self.t -= gone
 
-    def attend_group(self, query, key, value, scale: float):
+    def attend_group(self, query, key, value, scale: float, attention_mask=None):
         """A pass of n tokens after the prompt: [B,H,n,Dh] q/k/v -> [B,H,n,Dh]; appends them from slot t on."""
         if not self._pending:
             raise RuntimeError("FFACache: attend_group() without pending tokens")
         dt, n = self.dtype, key.shape[-2]
+        parents = self._note_group_mask(attention_mask, n)
         q, k, v = query.to(dt), key.to(dt), value.to(dt)
         k_cache, v_cache = self.engine.get_cache()
         outs = []
         for i in range(0, n, 64):
             part = slice(i, min(n, i + 64))
             outs.append(self.engine.attention_tree(q[:, :, part], k[:, :, part], v[:, :, part], k_cache, v_cache,
-                                                   float(scale), self.t + i, first_keys=self.first_key))
+                                                   float(scale), self.t + i, None if parents is None else parents[:, part] - i,
+                                                   first_keys=self.first_key))
         self.t += n
         self.seen += n
         self._pending = False
@@ -333,6 +385,14 @@ def enabled_by_env() -> bool:
 
 
 # -- attention hooks --------------------------------------------------------------------------
+def _visible(mask):
+    """Where an attention mask lets a key through: True, a whole number other than 0, or a float that is no
+    large negative number (transformers masks with the type's lowest)."""
+    if mask.dtype == torch.bool:
+        return mask
+    return mask > -1e4 if mask.dtype.is_floating_point else mask != 0
+
+
 def _plain_attention(query, key, value, attention_mask, scaling):
     """Ordinary masked softmax attention for the prompt pass: [B,H,Lq,Dh] and the weights [B,H,Lq,Lk]."""
     w = torch.matmul(query, key.transpose(-1, -2)) * scaling
@@ -349,8 +409,8 @@ def ffa_attention_forward(module, query, key, value, attention_mask, scaling=Non
         scaling = query.shape[-1] ** -0.5
     layer = getattr(key, _TAG, None)
     if layer is not None and layer._pending:
-        if query.shape[-2] > 1:
-            return layer.attend_group(query, key, value, scaling).transpose(1, 2).contiguous(), None
+        if layer.takes_group(query.shape[-2]):
+            return layer.attend_group(query, key, value, scaling, attention_mask).transpose(1, 2).contiguous(), None
         return layer.attend(query, key, value, scaling).unsqueeze(1), None
     if layer is not None:
         layer.note_prompt_mask(attention_mask)
@@ -364,8 +424,8 @@ def _gptj_attn(self, query, key, value, attention_mask=None, *rest):
     """Replacement for GPTJAttention._attn (modeling_gptj.py:252-281): ([B,H,Lq,Dh], weights)."""
     layer = getattr(key, _TAG, None)
     if layer is not None and layer._pending:
-        if query.shape[-2] > 1:
-            return layer.attend_group(query, key, value, 1.0 / self.scale_attn), None
+        if layer.takes_group(query.shape[-2]):
+            return layer.attend_group(query, key, value, 1.0 / self.scale_attn, attention_mask), None
         return layer.attend(query, key, value, 1.0 / self.scale_attn).unsqueeze(2), None
     if layer is not None:
         layer.note_prompt_mask(attention_mask)
@@ -384,7 +444,7 @@ def _gptj_forward(self, hidden_states, layer_past=None, attention_mask=None, pos
     if isinstance(layer_past, FFACache) and self.layer_idx is not None and len(layer_past.layers) > self.layer_idx:
         layer = layer_past.layers[self.layer_idx]
     # The engine rotates by the slot's distance from the first key: not the token's position after an eviction.
-    if (layer is None or layer.engine is None or layer.bounded is not None or hidden_states.shape[1] != 1
+    if (layer is None or layer.engine is None or layer.bounded is not None or layer.takes_group(hidden_states.shape[1])
             or output_attentions or not hasattr(layer.engine, "attention_ex")):
         return self._ffa_original_forward(hidden_states, layer_past, attention_mask, position_ids, use_cache,
                                           output_attentions, **kwargs)
