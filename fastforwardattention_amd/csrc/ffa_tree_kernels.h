@@ -33,8 +33,8 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 // Scores may exceed a row's reference exponent by kSlack; a rescaled row starts at 2^kLift.  In
-// fp16 the range of P is what these two set: below 65504 at the top, and a weight of 2^-30 of the
-// row's largest is still above half the smallest number.
+// fp16 the range of P is what these two set: below 65504 at the top, and the smallest number, below which
+// weights are dropped, is 2^-30 of the row's largest.
 constexpr float kSlack = 15.f, kLift = 6.f;
 
 // Geometry of one element type, head dimension and number of row tiles.
@@ -66,10 +66,11 @@ __device__ __forceinline__ f32x4_t mma_qk(const uint4& k, const uint4& q, f32x4_
     return acc;
 }
 
-// The weights of one row tile as right operands.  16-bit types: P = hi + lo, hi rounded towards
-// zero, so that the weights are off by 2^-20 (fp16) or 2^-14 (bf16) at most and the result is as
-// good as with fp32 weights after its own rounding to 11 or 8 bits.  lo is kept above zero: 0 * V would turn an infinite
-// V into NaN.  (A NaN weight is NaN in hi, whatever lo is.)
+// The weights of one row tile as right operands.  16-bit types: P = hi + lo, both rounded towards
+// zero, so that a weight is off by 2^-20 (fp16) or 2^-14 (bf16) of itself, or in fp16 by 2^-24, which is
+// 2^-30 of the row's largest, whichever is more; the result's own rounding is to 11 or 8 bits.  Where hi is
+// above zero lo is too: 0 * V would turn an infinite V into NaN.  Where hi is zero lo is zero: what has no weight,
+// or is masked, adds nothing, however large its V.  (A NaN weight is NaN in hi, whatever lo is.)
 struct PFrag16 { uint4 hi, lo; };
 typedef __fp16 fp16x2_t __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
@@ -80,8 +81,11 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint3
     float ra, rb;
     asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(h), "v"(a));
     asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(h), "v"(b));
-    const half2_t rest = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(ra, rb));
-    const half2_t tiny = __builtin_bit_cast(half2_t, 0x00010001u);  // 2^-24, the smallest fp16
+    const u16x2_t rest = __builtin_bit_cast(u16x2_t, __builtin_amdgcn_cvt_pkrtz(ra, rb));
+    // Neither part is negative: their bit patterns order as they do.  1 is 2^-24, the smallest fp16.
+    u16x2_t one = {1, 1};
+    asm("" : "+s"(one));  // a known 1 becomes two comparisons, five instructions in place of one
+    const u16x2_t tiny = __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, h), one);
     *lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(rest, tiny));
 }
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint32_t* lo, bf16_t) {
@@ -89,8 +93,8 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint3
     *hi = __builtin_amdgcn_perm(ub, ua, 0x07060302);
     const float la = a - __builtin_bit_cast(float, ua & 0xffff0000u), lb = b - __builtin_bit_cast(float, ub & 0xffff0000u);
     const uint32_t rest = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, lb), __builtin_bit_cast(uint32_t, la), 0x07060302);
-    // The rest is not negative: its bit pattern orders as it does.  0x3380 is 2^-24.
-    const u16x2_t tiny = {0x3380, 0x3380};
+    // 0x0080 is 2^-126, the smallest normal number.
+    const u16x2_t tiny = __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, *hi), u16x2_t{0x0080, 0x0080});
     *lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, rest), tiny));
 }
 

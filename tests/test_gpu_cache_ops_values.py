@@ -1,0 +1,76 @@
+"""GPU tests of what values may do in the tree attention and the weight-summing step: large finite values of
+keys without weight, and NaN keys, wherever the cut of the keys puts them."""
+import pytest
+import torch
+
+from tests.cache_ops_testlib import DEV, DT, pack_k, pack_v, random_parents
+from tests.test_gpu_cache_ops import FFA, INF, NAN, ints, make
+
+pytestmark = pytest.mark.gpu
+
+LARGE = {"fp16": 65504.0, "bf16": 3e38, "fp32": 3e38}
+
+
+def bits(x):
+    return x.contiguous().view(torch.int32 if x.dtype == torch.float32 else torch.int16)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("Dh", [64, 80, 128, 256])
+@pytest.mark.parametrize("t,n,G", [(0, 2, 1), (70, 40, 2), (5000, 33, 1), (1300, 64, 4)])
+def test_large_values_of_nodes_out_of_sight(dtype, Dh, t, n, G):
+    """Rows that do not see a node come out the same, bit for bit, whatever finite value it holds."""
+    print("out of sight", dtype, Dh, t, n, G, flush=True)
+    H = 2
+    g, kc, vc, q, k, v = make(t + n, dtype, 1, H, H * G, Dh, t, n)
+    siblings = torch.tensor([[-1] + [0] * (n - 1)], dtype=torch.int32) if n > 2 else torch.tensor([[-1, -1]], dtype=torch.int32)
+    hidden = n // 2 if n > 2 else 0
+    for parents, rows in ((siblings, [i for i in range(n) if i != hidden]), (None, list(range(n - 1)))):
+        node = hidden if parents is not None else n - 1
+        got = []
+        for value in (0.0, LARGE[dtype], -LARGE[dtype]):
+            v2 = v.clone()
+            v2[:, :, node] = value
+            got.append(FFA().attention_tree(q, k, v2, kc, vc, Dh ** -0.5, t, ints(parents))[:, :, rows])
+        assert bool(got[0].isfinite().all())
+        assert torch.equal(bits(got[0]), bits(got[1])) and torch.equal(bits(got[0]), bits(got[2])), (parents is None)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("Dh", [64, 80, 128, 256])
+@pytest.mark.parametrize("t", [50, 5000])
+def test_large_values_of_cached_keys_without_weight(dtype, Dh, t):
+    """A cached key whose score lies so far below the others that its weight is 0 in 32 bits (e^-400) adds nothing."""
+    print("without weight", dtype, Dh, t, flush=True)
+    g, kc, vc, q, k, v = make(t, dtype, 2, 2, 2, Dh, t, 5)
+    K = torch.randn(2, 2, t, Dh, generator=g) * 0.1
+    K[..., 0] = 0
+    K[:, :, 3::7, 0] = -100
+    kc = pack_k(K.to(DT[dtype]).to(DEV), kc.shape[3], NAN)
+    q[..., 0], k[..., 0] = 4.0, 0.0
+    V = vc[:, :, :t].clone()
+    par = ints(random_parents(g, 2, 5))
+    got, summed = [], []
+    for value in (0.0, LARGE[dtype], -LARGE[dtype]):
+        V[:, :, 3::7] = value
+        vc = pack_v(V, kc.shape[3], NAN)
+        got.append(FFA().attention_tree(q, k, v, kc.clone(), vc.clone(), 1.0, t, par))
+        w = torch.zeros(2, 2, kc.shape[3], device=DEV)
+        summed.append(FFA().attention_weights(q[:, :, 0].contiguous(), k[:, :, 0].contiguous(), v[:, :, 0].contiguous(), kc.clone(), vc, 1.0, t, w))
+        assert not bool(w[:, :, 3:t:7].any())
+    for x in (got, summed):
+        assert bool(x[0].isfinite().all()) and torch.equal(bits(x[0]), bits(x[1])) and torch.equal(bits(x[0]), bits(x[2]))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+def test_infinite_values_of_light_keys(dtype):
+    """A visible infinite value shows, also behind a weight whose lower part is zero."""
+    print("light", dtype, flush=True)
+    _, kc, vc, q, k, v = make(15, dtype, 1, 1, 1, 64, 64, 1)
+    kc = pack_k(torch.zeros(1, 1, 64, 64, dtype=DT[dtype], device=DEV), kc.shape[3], NAN)
+    k = torch.zeros_like(k)
+    for slot in range(0, 64, 9):
+        vc2 = vc.clone()
+        vc2[0, 0, slot, 5] = INF
+        out = FFA().attention_tree(q, k, v, kc, vc2, 0.125, 64)
+        assert float(out[0, 0, 0, 5]) == INF and bool(out[0, 0, 0, :5].isfinite().all()) and bool(out[0, 0, 0, 6:].isfinite().all())
