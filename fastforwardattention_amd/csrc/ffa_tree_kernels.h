@@ -653,7 +653,8 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT)) ffa_tree_
         const int row = row0 + tid;
         if ((!whole || weights) && row < P.rows) {
             float* to = P.ws_ml + (((size_t)pair * n_splits + split) * P.rows + row) * 2;
-            to[0] = M;
+            // A maximum of -infinity says that the piece holds nothing; one of NaN scores alone has that too.
+            to[0] = M == -INFINITY && L != 0.f ? 0.f : M;
             to[1] = L;
         }
     }

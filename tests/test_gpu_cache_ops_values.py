@@ -74,3 +74,38 @@ def test_infinite_values_of_light_keys(dtype):
         vc2[0, 0, slot, 5] = INF
         out = FFA().attention_tree(q, k, v, kc, vc2, 0.125, 64)
         assert float(out[0, 0, 0, 5]) == INF and bool(out[0, 0, 0, :5].isfinite().all()) and bool(out[0, 0, 0, 6:].isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("where", ["a run of keys", "one key behind padding", "one key before the end"])
+def test_nan_scores_show_whatever_piece_they_fill(dtype, where):
+    """A row that sees a NaN key is NaN, and so are the weights it gives, also where the keys are cut in pieces
+    and all that the row sees of a piece is NaN.  The sample beside it has none."""
+    print("NaN piece", dtype, where, flush=True)
+    t, H, Dh = 6000, 2, 64
+    _, kc, vc, q, k, v = make(16, dtype, 2, H, H, Dh, t, 3)
+    first, lengths = [0, 0], [t, t]
+    if where == "a run of keys":
+        nan = slice(500, 5500)                     # whole pieces, and none of the first and the last
+    elif where == "one key behind padding":
+        first[0] = t - 200
+        nan = slice(first[0], first[0] + 1)
+    else:
+        lengths[0] = 3001
+        nan = slice(3000, 3001)
+    for at in {nan.start, nan.stop - 1, (nan.start + nan.stop) // 2}:
+        # Every cut: the visible keys of sample 0 end or begin at the NaN ones in one of these.
+        for f0, n0 in ((first[0], lengths[0]), (at, lengths[0]), (first[0], at + 1)):
+            if not f0 <= at < n0:
+                continue
+            kc2 = kc.clone()
+            kc2[0, 0, :, nan] = NAN
+            fk, ln = ints([f0, first[1]]), ints([n0, lengths[1]])
+            out = FFA().attention_tree(q, k, v, kc2, vc.clone(), 0.125, t, first_keys=fk, lengths=ln)
+            assert bool(out[0, 0].isnan().all()) and bool(out[0, 1].isfinite().all()) and bool(out[1].isfinite().all()), (at, f0, n0)
+            w = torch.zeros(2, H, kc.shape[3], device=DEV)
+            one = FFA().attention_weights(q[:, :, 0].contiguous(), k[:, :, 0].contiguous(), v[:, :, 0].contiguous(), kc2, vc.clone(), 0.125, t, w,
+                                          first_keys=fk, lengths=ln)
+            assert bool(one[0, 0].isnan().all()) and bool(one[0, 1].isfinite().all()) and bool(one[1].isfinite().all()), (at, f0, n0)
+            assert bool(w[0, 0, f0:n0 + 1].isnan().all()) and bool(w[0, 1].isfinite().all()) and bool(w[1].isfinite().all())
+            assert not bool(w[0, 0, :f0].any()) and not bool(w[0, 0, n0 + 1:].any())
