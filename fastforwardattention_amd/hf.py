@@ -265,16 +265,12 @@ class FFALayer(CacheLayerMixin):
         node = torch.arange(n, device=mask.device)
         return torch.where(node == first[:, None] - self.t, -1, node - 1).to(torch.int32)
 
-    def note_prompt_weights(self, weights):
-        """The prompt pass's attention weights [B,H,Lq,Lk], for a bounded cache: what each key received
-        from real queries.  Moves the prompt into the bounded caches."""
+    def note_prompt_weights(self, query, key, attention_mask, scaling):
+        """What each key of the prompt received from real queries, for a bounded cache.  Moves the prompt
+        into the bounded caches."""
         if self.keep is None:
             return
-        w = weights.float()
-        if self.first_key is not None:      # the rows of padding say nothing
-            real = torch.arange(w.shape[2], device=w.device)[None] >= self.first_key[:, None]
-            w = torch.where(real[:, None, :, None], w, 0.0)
-        w = w.sum(2).contiguous()
+        w = _prompt_weights(query, key, attention_mask, scaling, self.first_key)
         k, v = self.engine.get_cache()
         cap = self.keep + self.evict_every
         self.bounded = (k.new_empty((*k.shape[:3], cap, k.shape[4])), v.new_empty((*v.shape[:2], cap, v.shape[3])),
@@ -393,13 +389,36 @@ def _visible(mask):
     return mask > -1e4 if mask.dtype.is_floating_point else mask != 0
 
 
+def _masked(w, mask):
+    if mask is None:
+        return w
+    return w + mask if mask.dtype != torch.bool else w.masked_fill(~mask, float("-inf"))
+
+
 def _plain_attention(query, key, value, attention_mask, scaling):
-    """Ordinary masked softmax attention for the prompt pass: [B,H,Lq,Dh] and the weights [B,H,Lq,Lk]."""
-    w = torch.matmul(query, key.transpose(-1, -2)) * scaling
-    if attention_mask is not None:
-        w = w + attention_mask if attention_mask.dtype != torch.bool else w.masked_fill(~attention_mask, float("-inf"))
+    """Ordinary masked softmax attention for the prompt pass: [B,H,Lq,Dh]."""
+    w = _masked(torch.matmul(query, key.transpose(-1, -2)) * scaling, attention_mask)
     w = torch.softmax(w, dim=-1, dtype=torch.float32).to(value.dtype)
-    return torch.matmul(w, value), w
+    return torch.matmul(w, value)
+
+
+_WEIGHT_ROWS = 256      # queries at a time: bounds the scores held at once
+
+
+def _prompt_weights(query, key, attention_mask, scaling, first_key):
+    """The attention each key of the prompt receives, summed over the queries: float32 [B,H,Lk].  Scores and
+    probabilities are float32 too, as in the steps that add to these sums."""
+    q, kt = query.float(), key.float().transpose(-1, -2)
+    total = q.new_zeros((*q.shape[:2], kt.shape[-1]))
+    for i in range(0, q.shape[2], _WEIGHT_ROWS):
+        part = slice(i, min(i + _WEIGHT_ROWS, q.shape[2]))
+        mask = attention_mask if attention_mask is None or attention_mask.shape[-2] == 1 else attention_mask[..., part, :]
+        w = torch.softmax(_masked(torch.matmul(q[:, :, part], kt) * scaling, mask), dim=-1)
+        if first_key is not None:           # the rows of padding say nothing
+            real = torch.arange(part.start, part.stop, device=w.device)[None] >= first_key[:, None]
+            w = torch.where(real[:, None, :, None], w, 0.0)
+        total += w.sum(2)
+    return total
 
 
 def ffa_attention_forward(module, query, key, value, attention_mask, scaling=None, dropout=0.0, **kwargs):
@@ -414,9 +433,9 @@ def ffa_attention_forward(module, query, key, value, attention_mask, scaling=Non
         return layer.attend(query, key, value, scaling).unsqueeze(1), None
     if layer is not None:
         layer.note_prompt_mask(attention_mask)
-    out, weights = _plain_attention(query, key, value, attention_mask, scaling)
+    out = _plain_attention(query, key, value, attention_mask, scaling)
     if layer is not None:
-        layer.note_prompt_weights(weights)
+        layer.note_prompt_weights(query, key, attention_mask, scaling)
     return out.transpose(1, 2).contiguous(), None
 
 
@@ -431,7 +450,7 @@ def _gptj_attn(self, query, key, value, attention_mask=None, *rest):
         layer.note_prompt_mask(attention_mask)
     out, weights = self._ffa_original_attn(query, key, value, attention_mask, *rest)
     if layer is not None:
-        layer.note_prompt_weights(weights)
+        layer.note_prompt_weights(query, key, attention_mask, 1.0 / self.scale_attn)
     return out, weights
 
 
