@@ -66,13 +66,14 @@ __device__ __forceinline__ f32x4_t mma_qk(const uint4& k, const uint4& q, f32x4_
     return acc;
 }
 
-// The weights of one row tile as right operands.  16-bit types: P = hi + lo, both rounded towards
-// zero, so that a weight is off by 2^-20 (fp16) or 2^-14 (bf16) of itself, or in fp16 by 2^-24, which is
-// 2^-30 of the row's largest, whichever is more; the result's own rounding is to 11 or 8 bits.  Where hi is
+// The weights of one row tile as right operands.  16-bit types: P = hi + lo, hi rounded towards zero, so
+// that lo is not negative, lo to nearest: a weight is off by 2^-22 (fp16) or 2^-16 (bf16) of itself, or in fp16 by
+// 2^-24, which is 2^-30 of the row's largest, whichever is more; the result's own rounding is to 11 or 8 bits.  Where hi is
 // above zero lo is too: 0 * V would turn an infinite V into NaN.  Where hi is zero lo is zero: what has no weight,
 // or is masked, adds nothing, however large its V.  (A NaN weight is NaN in hi, whatever lo is.)
 struct PFrag16 { uint4 hi, lo; };
-typedef __fp16 fp16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint32_t* lo, uint16_t) {
     const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
@@ -81,7 +82,7 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint3
     float ra, rb;
     asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(h), "v"(a));
     asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(h), "v"(b));
-    const u16x2_t rest = __builtin_bit_cast(u16x2_t, __builtin_amdgcn_cvt_pkrtz(ra, rb));
+    const u16x2_t rest = __builtin_bit_cast(u16x2_t, __builtin_convertvector(f32x2_t{ra, rb}, half2_t));
     // Neither part is negative: their bit patterns order as they do.  1 is 2^-24, the smallest fp16.
     u16x2_t one = {1, 1};
     asm("" : "+s"(one));  // a known 1 becomes two comparisons, five instructions in place of one
@@ -92,10 +93,10 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint3
     const uint32_t ua = __builtin_bit_cast(uint32_t, a), ub = __builtin_bit_cast(uint32_t, b);
     *hi = __builtin_amdgcn_perm(ub, ua, 0x07060302);
     const float la = a - __builtin_bit_cast(float, ua & 0xffff0000u), lb = b - __builtin_bit_cast(float, ub & 0xffff0000u);
-    const uint32_t rest = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, lb), __builtin_bit_cast(uint32_t, la), 0x07060302);
+    const u16x2_t rest = __builtin_bit_cast(u16x2_t, __builtin_convertvector(f32x2_t{la, lb}, bf16x2_t));
     // 0x0080 is 2^-126, the smallest normal number.
     const u16x2_t tiny = __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, *hi), u16x2_t{0x0080, 0x0080});
-    *lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, rest), tiny));
+    *lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(rest, tiny));
 }
 
 template <typename T> __device__ __forceinline__ PFrag16 split_weights(const float* p, T tag) {
@@ -775,7 +776,6 @@ constexpr int kFinishKeys = 4;  // keys a thread
 template <typename T, int DH>
 __global__ void __launch_bounds__(256) ffa_tree_finish_kernel(const float* ws_acc, const float* ws_ml, int n_splits, int rows,
                                                               int join_blocks, const TreeParams P) {
-    typedef float f32x2_t __attribute__((ext_vector_type(2)));
     const int pairs = P.B * P.H;
     for (int pair = blockIdx.y; pair < pairs; pair += gridDim.y) {
         if ((int)blockIdx.x < join_blocks) {

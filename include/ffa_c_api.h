@@ -313,8 +313,8 @@ int ffa_load_floor(int precision, int batch_size, int head_num, int head_dim, in
  *   out[b,hq,i] = sum over j of softmax_j(softmax_scale <q[b,hq,i], k_j>) v_j,
  *   j = cached slots first .. length - 1 and node i with its ancestors.
  * Node i of sample b is appended at cache slot length + i.  Sums and softmax statistics are fp32;
- * in 16-bit types a weight enters the matrix products as a sum of two 16-bit numbers, off by 2^-20
- * (fp16) or 2^-14 (bf16) of itself, in fp16 also by up to 2^-30 of the row's largest; a weight of 0 adds
+ * in 16-bit types a weight enters the matrix products as a sum of two 16-bit numbers, off by 2^-22
+ * (fp16) or 2^-16 (bf16) of itself, in fp16 also by up to 2^-30 of the row's largest; a weight of 0 adds
  * nothing.
  *   tokens      nodes a sample, 1 .. FFA_MAX_TREE_TOKENS; t + tokens <= max_seq_len;
  *   q_head_num  a multiple G * head_num of the cache's heads: query head hq reads head hq / G;

@@ -109,3 +109,31 @@ def test_nan_scores_show_whatever_piece_they_fill(dtype, where):
             assert bool(one[0, 0].isnan().all()) and bool(one[0, 1].isfinite().all()) and bool(one[1].isfinite().all()), (at, f0, n0)
             assert bool(w[0, 0, f0:n0 + 1].isnan().all()) and bool(w[0, 1].isfinite().all()) and bool(w[1].isfinite().all())
             assert not bool(w[0, 0, :f0].any()) and not bool(w[0, 0, n0 + 1:].any())
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_weights_keep_two_16_bit_parts_rounded_to_nearest(dtype):
+    """Two keys whose values cancel but for 2^-9 (bf16) of the lighter one's weight p, so that the result's own rounding is
+    small.  The heavier key's weight is a power of two and exact.  p = 1.m splits into a part cut after 7 (bf16) or 10
+    (fp16) bits of m and the nearest number of 8 or 11 bits to the rest: 2^-16 or 2^-22 of p at most.  The scores are
+    single products; their scaling, the exponentials and the sum of the weights are 8 roundings of 2^-24, and the sums
+    of products as many."""
+    print("two parts", dtype, flush=True)
+    B, H, Dh = 4, 64, 64
+    g = torch.Generator().manual_seed(17)
+    dt = DT[dtype]
+    K, V = torch.zeros(B, H, 2, Dh), torch.zeros(B, H, 2, Dh)
+    K[:, :, 1, 0] = -0.1 - 0.55 * torch.rand(B, H, generator=g)
+    K = K.to(dt)
+    p = torch.exp(K[:, :, 1, 0].double())
+    V[:, :, 1], V[:, :, 0] = 1.0, -p[..., None].float()
+    V = V.to(dt)
+    q, k, v = (torch.zeros(B, H, 1, Dh, dtype=dt) for _ in range(3))
+    q[..., 0], k[..., 0] = 1.0, -100.0
+    want = (V[:, :, 0].double() + p[..., None] * V[:, :, 1].double()) / (1 + p[..., None])
+    kc, vc = pack_k(K.to(DEV), 4, NAN), pack_v(V.to(DEV), 4, NAN)
+    out = FFA().attention_tree(q.to(DEV), k.to(DEV), v.to(DEV), kc, vc, 1.0, 2)[:, :, 0].double().cpu()
+    part = 2.0 ** -16 if dtype == "bf16" else 2.0 ** -22
+    tol = torch.finfo(dt).eps / 2 * want.abs() + ((part + 16 * 2.0 ** -24) * p / (1 + p))[..., None]
+    assert float(tol.max()) < 2.0 ** -16
+    assert bool(((out - want).abs() <= tol).all()), float(((out - want).abs() / tol).max())
