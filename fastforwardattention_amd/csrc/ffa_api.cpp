@@ -135,7 +135,7 @@ const char* ffa_status_string(int status) {
         case FFA_ERR_TRANSFORM: return "bad token transform: rotary dimension must be even and within [0, head_dim], biases 16-byte aligned";
         case FFA_ERR_TREE: return "bad group of new tokens: 1 to 64 of them, t + tokens <= max_seq_len, query heads a multiple of the cache's heads, strides multiples of 16 bytes";
         case FFA_ERR_EVICT: return "bad eviction: keep must be at least 1 and fit the target, recent must be within [0, keep]";
-        case FFA_ERR_OVERLAP: return "caches of a commit overlap, or an eviction target overlaps another buffer of the call without being its own source";
+        case FFA_ERR_OVERLAP: return "caches of a commit overlap, or an eviction's target or list of kept slots overlaps another buffer of the call (a target may be its own source)";
         case FFA_ERR_SCRATCH_LIMIT: return "the launch plan needs more scratch than the library's static 4 MiB array holds";
         default: return "unknown status";
     }

@@ -310,7 +310,12 @@ int ffa_evict(int precision, int n_caches, const void* const* k_src, const void*
     }
     // Every target against every other buffer of the call: its own source may be the same buffer of the same shape.
     const bool same_shape = src_max_seq_len == dst_max_seq_len;
+    const size_t kept_bytes = (size_t)n_caches * pairs * keep * 4;
     for (int i = 0; i < n_caches; ++i) {
+        // The list of kept slots is written while other pairs' weights are still read.
+        if (overlap(k_src[i], src_kv, kept, kept_bytes) || overlap(v_src[i], src_kv, kept, kept_bytes) ||
+            overlap(w_src[i], src_w, kept, kept_bytes))
+            return FFA_ERR_OVERLAP;
         const void* dst[3] = {k_dst[i], v_dst[i], w_dst[i]};
         for (int a = 0; a < 3; ++a) {
             const size_t na = a == 2 ? dst_w : dst_kv;
@@ -324,7 +329,7 @@ int ffa_evict(int precision, int n_caches, const void* const* k_src, const void*
                     if (!own && overlap(dst[a], na, dst2[b], b == 2 ? dst_w : dst_kv)) return FFA_ERR_OVERLAP;
                 }
             }
-            if (overlap(dst[a], na, kept, (size_t)n_caches * pairs * keep * 4)) return FFA_ERR_OVERLAP;
+            if (overlap(dst[a], na, kept, kept_bytes)) return FFA_ERR_OVERLAP;
         }
     }
     const int most = launch_caches((long long)pairs);

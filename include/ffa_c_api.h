@@ -58,7 +58,8 @@ typedef enum ffa_status {
     FFA_ERR_EVICT = 17,         /* eviction: keep < 1 or past the target, recent outside      */
                                 /* [0, keep]                                                  */
     FFA_ERR_OVERLAP = 18        /* two caches of a commit overlap, or an eviction's target    */
-                                /* overlaps another buffer and is not exactly its own source  */
+                                /* overlaps another buffer and is not exactly its own source, */
+                                /* or its list of kept slots overlaps a buffer                */
 } ffa_status;
 
 /* precision codes: the same integers the reference passes to get_launch_params
@@ -396,7 +397,8 @@ int ffa_attention_weights(int precision, int batch_size, int head_num, int q_hea
  *   *_src, *_dst  HOST arrays of device pointers; a target is its own source (in place, same
  *                 max_seq_len) or overlaps no other buffer of the call, each of k, v and w by itself;
  *   w_src, w_dst  key_weights [B, H, src_max_seq_len] / [B, H, dst_max_seq_len];
- *   kept          device int32 [n_caches, B, H, keep]: the old slot of each kept one, -1 behind.
+ *   kept          device int32 [n_caches, B, H, keep]: the old slot of each kept one, -1 behind; overlaps
+ *                 no other buffer of the call.
  */
 int ffa_evict(int precision, int n_caches, const void* const* k_src, const void* const* v_src,
               const float* const* w_src, void* const* k_dst, void* const* v_dst, float* const* w_dst,
