@@ -61,13 +61,19 @@ struct TreeShape {
 };
 
 // 16-row tiles a workgroup may hold: more read the keys less often, but leave fewer waves a SIMD and cost more
-// before the first key and after the last.  Measured, us with two and with four, fp16 (B x H x Dh, 64 rows):
-//   one, where all workgroups of one tile run at once: 1x32x128 t 1000 15 and 24 (2 pairs, 472 rows, Dh 256 one 14,
-//   two 21); two up to 1280 keys: 8x32x128 t 512 23 and 28, t 1000 38 and 40, t 2000 84 and 71;
-//   four of 16-bit Dh 64, two of whose workgroups fit a CU, where there are more: 16x32x64 t 0 17.7 and 14.1, t 600
-//   33 and 29, t 4000 150 and 103 (8x32x64 t 0 10.3 and 11.5);
-//   two of Dh 80, whose tiles take as many registers as Dh 96 would: 16x32x80 t 1000 52 and 69, 2x8(64) t 4000 35
-//   and 46, but 1x32 t 4000 33 and 25.
+// before the first key and after the last.  Measured, us in fp16 / bf16 / fp32, 64 rows (B x H x Dh):
+//   one, where all workgroups of one tile run at once on few keys, against two: 1x32x128 t 500 12 and 16 / 12 and 14 /
+//   19 and 22, t 1000 15 and 18 / 15 and 16 / 26 and 29; 1x32x256 t 1000 26 and 34 / 26 and 33 / 47 and 49; 1x32x80
+//   t 100, 32 rows 8.5 and 10.6 / 8.3 and 11.0 / 10.4 and 12.2 (64 rows from t 500 on alike or up to 20 % the other way);
+//   two up to 1280 keys, against four: 8x32x128 t 512 27 and 28 / 24 and 29 / 58 and 64, t 1280 43 and 43 / 39 and 45 /
+//   121 and 123, but t 4000 137 and 110 / 129 and 112 / 337 and 338 (about 1500 to 2500 keys two are still 5 to 15 %
+//   ahead); fp32 8x32x64 t 500 33 and 35, 11x32x64 t 800 59 and 77 (16x32x64 t 800 81 and 80);
+//   four of 16-bit Dh 64, two of whose workgroups fit a CU, where there are more, against two: 16x32x64 t 0 14 and 18 /
+//   14 and 18, t 600 28 and 33 / 28 and 33, t 4000 108 and 144 / 108 and 139 (8x32x64 t 0 10.9 and 9.6 / 11.5 and 9.9);
+//   two of Dh 80, whose tiles take as many registers as Dh 96 would, against four: 16x32x80 t 1000 51 and 68 / 52 and
+//   71 / 133 and 139, t 4000 166 and 164 / 163 and 169 / 450 and 444; 2x8(64) t 4000 35 and 46 / 36 and 48 / 108 and
+//   122.  With fewer tiles two win on 64 rows (1x32x80 t 4000 21 and 25 / 22 and 26 / 40 and 44) and lose on 33 to 48,
+//   which four read once (t 16000, 40 rows 41 and 39 / 41 and 40 / 114 and 88): four stay.
 int most_row_tiles(int precision, int head_dim, int t, long long tiles, int cus) {
     const int most = tree_row_tiles(head_dim);
     if (head_dim == 64 && elem_bytes(precision) == 2 && tiles > 4 * cus) return most;
