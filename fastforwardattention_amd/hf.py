@@ -125,7 +125,8 @@ class FFALayer(CacheLayerMixin):
 
     def _check_room(self, n):
         if self.seen + n > self.max_len:
-            raise RuntimeError(f"FFACache: cache full ({self.max_len} slots = prompt + max_new_tokens)")
+            raise RuntimeError(f"FFACache: cache full ({self.max_len} slots = first pass + max_new_tokens, which counts the rest of "
+                               "a prompt in chunks and guesses too)")
 
     def _check_group_pass(self):
         if self.beam_table is not None or self.bounded is not None or not hasattr(self.engine, "attention_tree"):
@@ -355,7 +356,8 @@ class FFALayer(CacheLayerMixin):
 class FFACache(Cache):
     """`past_key_values` object that keeps every layer's keys and values inside a
     `FastForwardAttn` (cache layouts [B,H,Dh/x,Lmax,x] / [B,H,Lmax,Dh], Lmax = prompt +
-    max_new_tokens).  `engine` replaces the `FastForwardAttn` class (same constructor and
+    max_new_tokens, which counts every token after the first pass: also the rest of a prompt fed in
+    chunks, and guesses that are taken back).  `engine` replaces the `FastForwardAttn` class (same constructor and
     methods); tests use it to run the bookkeeping without a GPU.  num_beams: generate's num_beams
     when beam search is used (samples are grouped num_beams at a time, as generate lays them out).
     keep: bound the cache: keep + evict_every slots a head; when they are full, `keep` stay: the last

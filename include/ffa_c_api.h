@@ -327,6 +327,7 @@ int ffa_load_floor(int precision, int batch_size, int head_num, int head_dim, in
  *   *_stride    element strides of (sample, head, token) of q, k, v and out; each row of
  *               head_dim elements is contiguous, strides are multiples of 16 bytes, and the token
  *               strides of k and v are not negative and below 64 MiB.
+ * out overlaps neither k, v nor the caches.
  * A slot that no node may see (padding, slots from length on, nodes that are no ancestors) has
  * no influence whatever it holds, infinities and NaN included.
  * workspace: ffa_tree_workspace_bytes() for the same arguments (a step with the same arguments and
