@@ -223,6 +223,7 @@ class FFALayer(CacheLayerMixin):
         self.first_key = first.reshape(-1).to(torch.int32).contiguous()
         self.max_first = int(self.first_key.max())
         if self.keep is not None and self.max_first >= self.t:
+            self.reset()
             raise NotImplementedError("FFACache: a bounded cache wants a real token of every sample in the prompt")
 
     def takes_group(self, n: int) -> bool:

@@ -168,6 +168,23 @@ def test_bounded_cache_wants_a_real_token_of_every_sample():
     hf.disable(model)
 
 
+def test_refused_prompt_leaves_the_bounded_cache_empty():
+    model = tiny_opt()
+    ids, mask = padded_batch()
+    gone = mask.clone()
+    gone[1] = 0
+    hf.enable(model)
+    cache = hf.FFACache(max_new_tokens=4, engine=PlainEngine, keep=9)
+    with torch.no_grad():
+        with pytest.raises(NotImplementedError, match="real token"):
+            model(input_ids=ids, attention_mask=gone, past_key_values=cache, use_cache=True)
+        assert cache.get_seq_length() == 0
+        got = model(input_ids=ids, attention_mask=mask, past_key_values=cache, use_cache=True).logits
+        hf.disable(model)
+        want = model(input_ids=ids, attention_mask=mask).logits
+    assert float((got - want)[mask.bool()].abs().max()) < 2e-4
+
+
 def test_engine_without_group_attention_still_takes_single_tokens():
     """A sample that is all padding so far, on an engine without attention_tree: its keys begin behind the prompt."""
     model = tiny_opt()
