@@ -5,8 +5,8 @@
 // Mathematics.  The rows of a (sample, cache head) pair are its tokens times its G query heads.
 // For a tile of keys:  S^T = K Q^T (keys x rows),  P = 2^(S c - m),  O^T += V^T P^T (dims x rows),
 // l += sum P, with c = softmax_scale * log2(e) and m one reference exponent a row.  Any m cancels
-// in O / l, so m is only moved when a score exceeds it by kSlack: then rows are rescaled so that
-// their largest P is 2^kLift.  Pieces (waves, workgroups) are joined by their (m, l, O).
+// in O / l, so m is only moved when a score exceeds it by `slack`: then rows are rescaled so that
+// their largest P is 2^lift.  Pieces (waves, workgroups) are joined by their (m, l, O).
 //
 // Layout.  No operand passes through LDS.  A 16-byte chunk of a K cache row holds 8 (4) dims of
 // one key, which is what one lane of a 16x16x32 (four 16x16x4) matrix product wants of its left
@@ -32,10 +32,13 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-// Scores may exceed a row's reference exponent by kSlack; a rescaled row starts at 2^kLift.  In
+// Scores may exceed a row's reference exponent by `slack`; a rescaled row starts at 2^lift.  In
 // fp16 the range of P is what these two set: below 65504 at the top, and the smallest number, below which
-// weights are dropped, is 2^-30 of the row's largest.
-constexpr float kSlack = 15.f, kLift = 6.f;
+// weights are dropped, is 2^-30 of the row's largest.  The other types' V has the exponents of the fp32 sums: there P
+// stays below 4, so that the sums are finite where 4 times the sum of all |V| is.  (Lower, they would be finite for
+// larger V, but the exponent's argument is rounded to 2^-24 of its size: at -29 that costs two bits of P.)
+template <typename T> struct TreeRange { static constexpr float slack = 2.f, lift = -7.f; };
+template <> struct TreeRange<uint16_t> { static constexpr float slack = 15.f, lift = 6.f; };
 
 // Geometry of one element type, head dimension and number of row tiles.
 template <typename T, int DH, int RT> struct TreeGeo {
@@ -279,6 +282,7 @@ template <typename T, int DH, int RT> constexpr int tree_q_floats() {
 template <typename T, int DH, int RT, int W, bool STREAM>
 __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT)) ffa_tree_kernel(TREE_HOT_DECL, const TreeParams P) {
     using G = TreeGeo<T, DH, RT>;
+    constexpr float kSlack = TreeRange<T>::slack, kLift = TreeRange<T>::lift;
     constexpr int NU = G::NU, TK = G::TK, KK = G::KK, NCH = G::NCH, DB = G::DB, NJ = 4 * NU;
     constexpr unsigned ROW = DH * sizeof(T);  // bytes of a cache row
     constexpr bool QLDS = tree_q_in_lds<T, DH, RT>();
@@ -682,12 +686,7 @@ __global__ void __launch_bounds__(W * 64, tree_waves_per_simd(DH, RT)) ffa_tree_
                                               : G::NBLK * 16 * G::E + gg * 4;
             f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
-                // A wave that counts nothing adds nothing, also where its sum is infinite.
-                const float f = s_ml[w][rt * 16 + r][0];
-                const f32x4_t x = s_acc[w * DB * 64 + i] * f;
-                o += f != 0.f ? x : f32x4_t{0.f, 0.f, 0.f, 0.f};
-            }
+            for (int w = 0; w < W; ++w) o += s_acc[w * DB * 64 + i] * s_ml[w][rt * 16 + r][0];
             const int token = quotient(row, P.G, P.G_magic);
             if (bad != 0) {
                 for (uint64_t todo = bad & s_seen[token]; todo != 0; todo &= todo - 1) {

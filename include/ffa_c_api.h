@@ -316,7 +316,7 @@ int ffa_load_floor(int precision, int batch_size, int head_num, int head_dim, in
  * Node i of sample b is appended at cache slot length + i.  Sums and softmax statistics are fp32;
  * in 16-bit types a weight enters the matrix products as a sum of two 16-bit numbers, off by 2^-22
  * (fp16) or 2^-16 (bf16) of itself, in fp16 also by up to 2^-30 of the row's largest; a weight of 0 adds
- * nothing.
+ * nothing.  In bf16 and fp32 4 times the sum of |v| over the keys has to be finite in fp32.
  *   tokens      nodes a sample, 1 .. FFA_MAX_TREE_TOKENS; t + tokens <= max_seq_len;
  *   q_head_num  a multiple G * head_num of the cache's heads: query head hq reads head hq / G;
  *   parents     [B, tokens]: the node's parent, a node before it; any value outside [0, i) makes

@@ -137,3 +137,54 @@ def test_weights_keep_two_16_bit_parts_rounded_to_nearest(dtype):
     tol = torch.finfo(dt).eps / 2 * want.abs() + ((part + 16 * 2.0 ** -24) * p / (1 + p))[..., None]
     assert float(tol.max()) < 2.0 ** -16
     assert bool(((out - want).abs() <= tol).all()), float(((out - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("Dh", [64, 80, 128, 256])
+@pytest.mark.parametrize("t,n", [(0, 1), (1, 3), (40, 40), (700, 5), (6000, 17)])
+def test_values_of_any_finite_size(dtype, Dh, t, n):
+    """All keys alike with weights 1 / keys and one value: the result is that value, also where 4 times the sum of the
+    values just fits fp32.  Bound: half a step, the two 16-bit parts, and 2 additions a key in numerator and sum."""
+    print("any size", dtype, Dh, t, n, flush=True)
+    B, H, dt = 1, 2, DT[dtype]
+    q, k = (torch.zeros(B, H, n, Dh, dtype=dt, device=DEV) for _ in range(2))
+    kc = pack_k(torch.zeros(B, H, t, Dh, dtype=dt, device=DEV), t + n + 1, NAN)
+    tol = torch.finfo(dt).eps / 2 + {"fp16": 2.0 ** -22, "bf16": 2.0 ** -16, "fp32": 0.0}[dtype] + (2 * (t + n) + 64) * 2.0 ** -24
+    large = 65504.0 if dtype == "fp16" else 8e37 / (t + n)
+    for value in (large, -large, 1.0, 0.01 if dtype == "fp16" else 1e-20):
+        V = torch.full((B, H, t + n, Dh), value, dtype=dt, device=DEV)
+        vc, v, x = pack_v(V[:, :, :t], t + n + 1, NAN), V[:, :, t:].clone(), float(V[0, 0, 0, 0])
+        w = torch.zeros(B, H, t + n + 1, device=DEV)
+        outs = [FFA().attention_tree(q, k, v, kc.clone(), vc.clone(), 1.0, t),
+                FFA().attention_weights(q[:, :, 0].contiguous(), k[:, :, 0].contiguous(), v[:, :, 0].contiguous(), kc.clone(), vc, 1.0, t, w)]
+        for out in outs:
+            # A result of fp16 that is rounded up past the largest number is infinite.
+            got = out.double().clamp(-65504, 65504) if dtype == "fp16" else out.double()
+            assert bool(((got - x).abs() <= tol * abs(x)).all()), (value, float((got - x).abs().max() / abs(x)), tol)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("Dh", [64, 80, 128, 256])
+@pytest.mark.parametrize("t,low", [(300, slice(0, 200)), (300, slice(100, 300)), (6000, slice(0, 4000)), (6000, slice(500, 6000)), (6000, slice(1000, 5000))])
+def test_large_values_of_a_stretch_without_weight(dtype, Dh, t, low):
+    """Whole tiles, waves and pieces whose keys have no weight (e^-400) next to the others: their values, as long as 4
+    times their sum fits fp32, change no bit, whichever come first; an infinite one shows."""
+    print("stretch", dtype, Dh, t, low, flush=True)
+    g, kc, vc, q, k, v = make(t + 1, dtype, 1, 2, 2, Dh, t, 5)
+    K = torch.randn(1, 2, t, Dh, generator=g) * 0.1
+    K[..., 0] = 0
+    K[:, :, low, 0] = -100
+    kc = pack_k(K.to(DT[dtype]).to(DEV), kc.shape[3], NAN)
+    q[..., 0], k[..., 0] = 4.0, 0.0
+    V = vc[:, :, :t].clone()
+    got, large = [], 65504.0 if dtype == "fp16" else 8e37 / t
+    for value in (0.0, large, -large, INF):
+        V[:, :, low] = value
+        vc = pack_v(V, kc.shape[3], NAN)
+        w = torch.zeros(1, 2, kc.shape[3], device=DEV)
+        got.append((FFA().attention_tree(q, k, v, kc.clone(), vc.clone(), 1.0, t),
+                    FFA().attention_weights(q[:, :, 0].contiguous(), k[:, :, 0].contiguous(), v[:, :, 0].contiguous(), kc.clone(), vc, 1.0, t, w)))
+    for i in range(2):
+        assert bool(got[0][i].isfinite().all())
+        assert torch.equal(bits(got[0][i]), bits(got[1][i])) and torch.equal(bits(got[0][i]), bits(got[2][i]))
+        assert not bool(got[3][i].isfinite().any())
